@@ -78,12 +78,12 @@ _STEM = int(os.environ.get("SPB_SPN_STEM", "1"))
 _FUSED_FC_UPDATE = os.environ.get("SPB_SPN_FUSED_FC_UPDATE", "0") == "1"
 
 
-def _low_priority_stream(device):
-    """lowest dispatch priority (spb_stream_create): its kernels take the compute units the launch stream leaves free.
-    SPB_SPN_UPDATE_PRIORITY = -1 / 0 / 1 overrides the level for experiments"""
+def _update_stream(device):
+    """the stream of the heads' update, at the default dispatch priority: streams of different priorities have hung on this hardware, and a
+    lower one made no measurable difference.  SPB_SPN_UPDATE_PRIORITY = -1 / 0 / 1 overrides the level for experiments"""
     h = C.c_void_p()
     with torch.cuda.device(device):
-        L.check(L.lib().spb_stream_create(int(os.environ.get("SPB_SPN_UPDATE_PRIORITY", "1")), C.byref(h)), "spb_stream_create")
+        L.check(L.lib().spb_stream_create(int(os.environ.get("SPB_SPN_UPDATE_PRIORITY", "0")), C.byref(h)), "spb_stream_create")
     return torch.cuda.ExternalStream(h.value, device=device)
 
 
@@ -525,7 +525,7 @@ class SpacecraftPoseNet(nn.Module):
         """the fully connected layers' weight gradient + parameter update kernels (SpnOptimizer.fused_fc_update) on a stream of
         their own, ordered after everything enqueued so far; the convolution weight gradients keep the side stream"""
         if getattr(self, "_upd", None) is None:
-            self._upd = _low_priority_stream(self._gflat.device)
+            self._upd = _update_stream(self._gflat.device)
         self._fork(self._upd)
         with torch.cuda.stream(self._upd):
             for name, gT, xT in jobs:
@@ -651,7 +651,7 @@ class SpacecraftPoseNet(nn.Module):
         """runs fn() (the heads' share of the optimizer step) on the update stream, ordered after everything enqueued so far; the next
         forward waits for it before fc6 (join_updates), state_dict() / flat_parameters() / invalidate() too"""
         if getattr(self, "_upd", None) is None:
-            self._upd = _low_priority_stream(self._gflat.device)
+            self._upd = _update_stream(self._gflat.device)
         self._fork(self._upd)
         with torch.cuda.stream(self._upd):
             fn()
@@ -816,7 +816,7 @@ class SpacecraftPoseNet(nn.Module):
                 # the convolution weight gradients keep the side stream.  Not earlier: the second head's chain streams its
                 # weights from HBM like the update does.
                 if getattr(self, "_upd", None) is None:
-                    self._upd = _low_priority_stream(self._gflat.device)
+                    self._upd = _update_stream(self._gflat.device)
                 self._fork(self._upd)
                 for sd in self._side_streams_in_use():
                     self._upd.wait_stream(sd)
