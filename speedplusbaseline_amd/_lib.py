@@ -13,6 +13,7 @@ if os.environ.get("SPB_LIB_VARIANT"):   # kernel experiments only (scratch/build
 F32, BF16 = 0, 1
 AMP_STATE, AMP_SCALE, AMP_INV_SCALE, AMP_TRACKER, AMP_FOUND_INF, AMP_STEPS, AMP_LR, AMP_SKIP = 12, 0, 1, 2, 3, 4, 5, 8   # spb_hip.h SPB_AMP_*
 ACT_NONE, ACT_RELU, ACT_RELU6, ACT_LEAKY = 0, 1, 2, 3
+ACT_GELU, ACT_GELU_TANH, ACT_SILU = 4, 5, 6   # spb_act8_* only
 
 vp = C.c_void_p
 fp = C.c_void_p  # float* passed as raw device address
@@ -246,6 +247,19 @@ SYMBOLS = {
     "spb_fc_epilogue": (i32, [C.POINTER(FcEpiArgs), vp]),
     "spb_spn_flatten": (i32, [vp, vp, vp, i32, i32, i32, vp]),
     "spb_spn_unflatten_grad": (i32, [vp, vp, i32, i32, i32, vp]),
+    # argument structs: _args8.py
+    "spb_layernorm_fwd": (i32, [i32, vp, vp]),
+    "spb_layernorm_bwd": (i32, [i32, vp, vp]),
+    "spb_layernorm_bwd_floats": (i64, [i64, i32]),
+    "spb_pack8_rows": (i32, [i32, vp, i64, i64, i32, vp, vp, vp]),
+    "spb_pack8_weight": (i32, [i32, vp, i64, i32, i32, vp, vp, vp, vp, vp]),
+    "spb_unpack8": (i32, [i32, vp, vp, i32, i64, i32, vp, i64, vp]),
+    "spb_act8_fwd": (i32, [i32, i32, vp, i64, vp, i64, i64, i32, vp, vp, vp]),
+    "spb_act8_bwd": (i32, [i32, i32, vp, i64, vp, vp, vp, i64, i64, i32, vp]),
+    "spb_gemm8": (i32, [i32, vp, vp]),
+    "spb_gemm8_bytes": (i64, [i32, i64, i32, i32]),
+    "spb_gemm8_wgrad": (i32, [i32, vp, vp]),
+    "spb_gemm8_wgrad_bytes": (i64, [i32, i64, i32, i32]),
     "spb_debug_trread": (i32, [vp, vp, vp]),
     "spb_version": (C.c_char_p, []),
     "spb_krn_num_acts": (i32, [vp]),

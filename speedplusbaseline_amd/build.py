@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libspb_hip.so")
 OBJDIR = os.path.join(HERE, "csrc", "_obj")
-SOURCES = ["gemm_pw.hip", "gemm_sk.hip", "gemm_os.hip", "gemm_big.hip", "gemm_rs.hip", "gemm_st.hip", "pw_bwd_fused.hip", "dwconv_rows.hip", "dwconv_plane.hip", "dwconv_tile.hip", "stem_head.hip", "stem_mfma.hip", "elemwise.hip", "ghiasi.hip", "ghiasi_wide.hip", "ghiasi_f32.hip", "spn.hip", "spn_fc.hip", "spn_conv.hip", "preproc.hip", "krn_plan.hip"]
+SOURCES = ["gemm_pw.hip", "gemm_sk.hip", "gemm_os.hip", "gemm_big.hip", "gemm_rs.hip", "gemm_st.hip", "pw_bwd_fused.hip", "dwconv_rows.hip", "dwconv_plane.hip", "dwconv_tile.hip", "stem_head.hip", "stem_mfma.hip", "elemwise.hip", "ghiasi.hip", "ghiasi_wide.hip", "ghiasi_f32.hip", "spn.hip", "spn_fc.hip", "spn_conv.hip", "preproc.hip", "krn_plan.hip",
+           "layernorm.hip", "pack8.hip", "gemm8.hip", "wgrad8.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value",
          # no packed float32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this hardware now and
          # then.  The host pass warns that it does not know the feature; that is harmless.
@@ -29,7 +30,9 @@ SOURCES_F16 = ["gemm_pw.hip", "elemwise.hip", "spn.hip", "spn_fc.hip", "spn_conv
                "stem_head.hip", "stem_mfma.hip", "krn_plan.hip",
                # round 6: the style decoder in IEEE half (Ghiasi(precision="fp16")): the reference runs this module in float32 (trainer.py:68-69);
                # half has eight times bfloat16's mantissa at the same matrix-core rate
-               "ghiasi.hip", "ghiasi_wide.hip", "ghiasi_f32.hip"]
+               "ghiasi.hip", "ghiasi_wide.hip", "ghiasi_f32.hip",
+               # layer norm and the 8-bit linear layers on float16 tensors
+               "layernorm.hip", "pack8.hip", "gemm8.hip", "wgrad8.hip"]
 # Reproducible twin (csrc/common.h, -DSPB_DET): the KRN / DANN kernels and the plan with exact (order-independent) accumulation in
 # place of float atomics.  KrnEngine(..., deterministic=True) and tests/test_parity_conditioned_gpu.py use it.
 # Tuning twin (-DSPB_TUNING): the only build that exports the spb_debug_set_* knobs (include/spb_hip_tuning.h).  Measurement scripts and

@@ -1,0 +1,440 @@
+// Layer norm over the last axis of [M, C] rows, forward and backward (spb_layernorm_* in include/spb_hip.h).
+//
+//   forward    mean = sum x / C,  var = sum (x - mean)^2 / C,  rstd = 1 / sqrt(var + eps),  y = (x - mean) rstd gamma + beta
+//   backward   h = g gamma,  xh = (x - mean) rstd:   dx = rstd (h - sum(h) / C - xh sum(h xh) / C)
+//              dgamma = sum over rows of g xh,  dbeta = sum over rows of g
+//
+// Both are bound by HBM: the forward reads x and writes y, the backward reads g and x and writes dx, each element once, because a row
+// stays in registers between its sums and its output.  The variance is taken from the differences to the mean, not from the sum of
+// squares: a row whose mean is far larger than its spread would lose the variance in the subtraction.  All sums are f32.
+//   * TPR threads share a row (16, 64 or 256), so that short rows fill a wave (four rows of up to 256 columns) and long rows need no second
+//     pass (8192 columns: 32 elements a thread).  Rows longer than that go through memory once per sum (ln_*_long).
+//   * Workgroups walk the rows with a stride, gamma and beta stay in registers, and the next row is requested before this one is summed.
+//   * dgamma / dbeta: a thread keeps its columns' sums in registers over its rows, the groups of a workgroup join through LDS, a workgroup
+//     stores one partial row, and a second launch adds the partial rows in order: no atomics, the same bits in every run.
+#include "common.h"
+
+namespace {
+
+constexpr int LN_REG_MAX = 8192;      // longest row held in registers
+constexpr int LN_FWD_WGS = 2048;      // workgroups that walk the rows: eight of 256 threads on each of the 256 compute units
+constexpr int LN_BWD_WGS = 512;       // backward: each stores one partial row of 2 C floats, so fewer of them
+
+// the 8 * NV elements of a row that a thread holds: vectors of 8 (VEC: 16-byte aligned rows and C % 8 == 0) or single elements a group apart
+template <typename T, int TPR, int NV, bool VEC> struct RowRegs {
+  Raw8<T> r[NV];
+  __device__ __forceinline__ void load(const T* row, int C, int lane) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * TPR + lane) * 8;
+      r[j] = ldraw<T>(row + (c < C ? c : 0));
+    }
+  }
+  __device__ __forceinline__ void get(float v[NV][8]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) cvt8(r[j], v[j]);
+  }
+};
+template <typename T, int TPR, int NV> struct RowRegs<T, TPR, NV, false> {
+  T e[NV][8];
+  __device__ __forceinline__ void load(const T* row, int C, int lane) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = (j * 8 + i) * TPR + lane;
+        e[j][i] = row[c < C ? c : 0];
+      }
+  }
+  __device__ __forceinline__ void get(float v[NV][8]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = to_f<T>(e[j][i]);
+  }
+};
+template <int TPR, bool VEC> __device__ __forceinline__ int ln_col(int j, int i, int lane) {
+  return VEC ? (j * TPR + lane) * 8 + i : (j * 8 + i) * TPR + lane;
+}
+template <int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_param(const float* p, float other, int C, int lane, float v[NV][8]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = ln_col<TPR, VEC>(j, i, lane);
+      v[j][i] = p != nullptr ? p[c < C ? c : 0] : other;
+    }
+}
+template <typename T, int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_store(T* row, int C, int lane, const float v[NV][8]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (VEC) {
+      const int c = (j * TPR + lane) * 8;
+      if (c < C) st8<T>(row + c, v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = (j * 8 + i) * TPR + lane;
+        if (c < C) row[c] = from_f<T>(v[j][i]);
+      }
+    }
+  }
+}
+
+// sums over the TPR threads of a row's group, in every thread of it.  TPR 256: `red` holds 4 floats for each value; the caller alternates
+// between buffers so that one barrier a reduction is enough.
+__device__ __forceinline__ float ln_wave_sum(float v) { return xor32_sum(xor16_sum(row16_sum(v))); }
+template <int TPR, int NVAL> __device__ __forceinline__ void group_sum(float v[NVAL], float* red) {
+#pragma unroll
+  for (int k = 0; k < NVAL; ++k) v[k] = TPR == 16 ? row16_sum(v[k]) : ln_wave_sum(v[k]);
+  if (TPR == 256) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < NVAL; ++k) red[k * 4 + w] = v[k];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < NVAL; ++k) v[k] = (red[k * 4] + red[k * 4 + 1]) + (red[k * 4 + 2] + red[k * 4 + 3]);
+  }
+}
+
+template <typename T, int TPR, int NV, bool VEC>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(const spb_layernorm_args_t a) {
+  constexpr int GR = 256 / TPR;                  // rows a workgroup works on at a time
+  __shared__ float red[4][4];
+  const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  const int C = a.C;
+  const float inv = 1.f / (float)C;
+  const T* X = reinterpret_cast<const T*>(a.X);
+  T* Y = reinterpret_cast<T*>(a.Y);
+  const long long step = (long long)gridDim.x * GR;
+  long long m = (long long)blockIdx.x * GR + grp;
+  RowRegs<T, TPR, NV, VEC> cur, nxt;
+  cur.load(X + (m < a.M ? m : a.M - 1) * a.ldx, C, lane);
+  float gm[NV][8], bt[NV][8];
+  ln_param<TPR, NV, VEC>(a.gamma, 1.f, C, lane, gm);
+  ln_param<TPR, NV, VEC>(a.beta, 0.f, C, lane, bt);
+  // TPR 256: m is the same in the whole workgroup, so is the trip count; the other groups of a wave may end a trip apart (no barrier there,
+  // and the DPP sums of a group read its own lanes only -- the loop runs until the last group of the WAVE is done)
+  const long long first = TPR == 256 ? m : (long long)blockIdx.x * GR + (threadIdx.x >> 6) * (64 / (TPR < 64 ? TPR : 64));
+  int flip = 0;
+  for (long long base = first; base < a.M; base += step, m += step, flip ^= 2) {
+    const long long mn = m + step;
+    nxt.load(X + (mn < a.M ? mn : a.M - 1) * a.ldx, C, lane);
+    float v[NV][8];
+    cur.get(v);
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[0] += ln_col<TPR, VEC>(j, i, lane) < C ? v[j][i] : 0.f;
+    group_sum<TPR, 1>(s, red[flip]);
+    const float mean = s[0] * inv;
+    float q[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[j][i] -= mean;
+        q[0] += ln_col<TPR, VEC>(j, i, lane) < C ? v[j][i] * v[j][i] : 0.f;
+      }
+    group_sum<TPR, 1>(q, red[flip + 1]);
+    const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * gm[j][i] + bt[j][i];
+    if (m < a.M) {
+      ln_store<T, TPR, NV, VEC>(Y + m * a.ldy, C, lane, v);
+      if (lane == 0) { a.mean[m] = mean; a.rstd[m] = rstd; }
+    }
+    cur = nxt;
+  }
+}
+
+// rows longer than LN_REG_MAX: a workgroup a row, the row read once for each sum and once for the output (from L2 after the first time)
+__device__ __forceinline__ float wg_sum(float v, float* red) {
+  v = ln_wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void ln_fwd_long(const spb_layernorm_args_t a) {
+  __shared__ float red[4];
+  const float inv = 1.f / (float)a.C;
+  for (long long m = blockIdx.x; m < a.M; m += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.X) + m * a.ldx;
+    T* y = reinterpret_cast<T*>(a.Y) + m * a.ldy;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < a.C; c += 256) s += to_f<T>(x[c]);
+    const float mean = wg_sum(s, red) * inv;
+    float q = 0.f;
+    for (int c = threadIdx.x; c < a.C; c += 256) { const float d = to_f<T>(x[c]) - mean; q += d * d; }
+    const float rstd = 1.f / sqrtf(wg_sum(q, red) * inv + a.eps);
+    for (int c = threadIdx.x; c < a.C; c += 256)
+      y[c] = from_f<T>((to_f<T>(x[c]) - mean) * rstd * (a.gamma ? a.gamma[c] : 1.f) + (a.beta ? a.beta[c] : 0.f));
+    if (threadIdx.x == 0) { a.mean[m] = mean; a.rstd[m] = rstd; }
+  }
+}
+
+template <typename T, int TPR, int NV, bool VEC, bool SUMS>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t a) {
+  constexpr int GR = 256 / TPR;
+  __shared__ float red[2][8];
+  __shared__ float join[SUMS && GR > 1 ? GR * TPR * NV * 8 : 1];
+  const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+  const int C = a.C;
+  const float inv = 1.f / (float)C;
+  const T* X = reinterpret_cast<const T*>(a.X);
+  const T* G = reinterpret_cast<const T*>(a.G);
+  T* D = reinterpret_cast<T*>(a.Y);
+  const long long step = (long long)gridDim.x * GR;
+  long long m = (long long)blockIdx.x * GR + grp;
+  RowRegs<T, TPR, NV, VEC> cx, cg, nx, ng;
+  float cm, cr, nm, nr;
+  {
+    const long long mc = m < a.M ? m : a.M - 1;
+    cx.load(X + mc * a.ldx, C, lane); cg.load(G + mc * a.ldg, C, lane);
+    cm = a.mean[mc]; cr = a.rstd[mc];
+  }
+  float gm[NV][8], dg[NV][8], db[NV][8];
+  ln_param<TPR, NV, VEC>(a.gamma, 1.f, C, lane, gm);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { dg[j][i] = 0.f; db[j][i] = 0.f; }
+  const long long first = TPR == 256 ? m : (long long)blockIdx.x * GR + (threadIdx.x >> 6) * (64 / (TPR < 64 ? TPR : 64));
+  int flip = 0;
+  for (long long base = first; base < a.M; base += step, m += step, flip ^= 1) {
+    const long long mn = m + step, mc = mn < a.M ? mn : a.M - 1;
+    nx.load(X + mc * a.ldx, C, lane); ng.load(G + mc * a.ldg, C, lane);
+    nm = a.mean[mc]; nr = a.rstd[mc];
+    float x[NV][8], g[NV][8];
+    cx.get(x); cg.get(g);
+    const bool row = m < a.M;
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = row && ln_col<TPR, VEC>(j, i, lane) < C;
+        x[j][i] = in ? (x[j][i] - cm) * cr : 0.f;           // xh
+        g[j][i] = in ? g[j][i] : 0.f;
+        if (SUMS) { dg[j][i] += g[j][i] * x[j][i]; db[j][i] += g[j][i]; }
+        g[j][i] *= gm[j][i];                                 // h
+        s[0] += g[j][i]; s[1] += g[j][i] * x[j][i];
+      }
+    group_sum<TPR, 2>(s, red[flip]);
+    const float s1 = s[0] * inv, s2 = s[1] * inv;
+    if (row) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[j][i] = cr * (g[j][i] - s1 - x[j][i] * s2);
+      ln_store<T, TPR, NV, VEC>(D + m * a.ldy, C, lane, g);
+    }
+    cx = nx; cg = ng; cm = nm; cr = nr;
+  }
+  if (SUMS) {
+    float* out = a.part + (size_t)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (GR > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) join[grp * (TPR * NV * 8) + ln_col<TPR, VEC>(j, i, lane)] = half ? db[j][i] : dg[j][i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += 256) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < GR; ++k) v += join[k * (TPR * NV * 8) + c];
+          out[half * C + c] = v;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int c = ln_col<TPR, VEC>(j, i, lane);
+            if (c < C) out[half * C + c] = half ? db[j][i] : dg[j][i];
+          }
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_long(const spb_layernorm_args_t a) {
+  __shared__ float red[4];
+  const float inv = 1.f / (float)a.C;
+  for (long long m = blockIdx.x; m < a.M; m += gridDim.x) {
+    const T* x = reinterpret_cast<const T*>(a.X) + m * a.ldx;
+    const T* g = reinterpret_cast<const T*>(a.G) + m * a.ldg;
+    T* d = reinterpret_cast<T*>(a.Y) + m * a.ldy;
+    const float mean = a.mean[m], rstd = a.rstd[m];
+    float s = 0.f, q = 0.f;
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const float h = to_f<T>(g[c]) * (a.gamma ? a.gamma[c] : 1.f);
+      s += h; q += h * (to_f<T>(x[c]) - mean) * rstd;
+    }
+    s = wg_sum(s, red) * inv;
+    q = wg_sum(q, red) * inv;
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const float h = to_f<T>(g[c]) * (a.gamma ? a.gamma[c] : 1.f);
+      d[c] = from_f<T>(rstd * (h - s - (to_f<T>(x[c]) - mean) * rstd * q));
+    }
+  }
+}
+// partial rows of dgamma / dbeta for long rows: a thread a column, blockIdx.y a range of rows.  It runs BEFORE ln_bwd_long, whose output may
+// overwrite g.
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_cols(const spb_layernorm_args_t a, long long rows) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  const long long m0 = (long long)blockIdx.y * rows, m1 = m0 + rows < a.M ? m0 + rows : a.M;
+  if (c >= a.C) return;
+  float dg = 0.f, db = 0.f;
+  for (long long m = m0; m < m1; ++m) {
+    const float g = to_f<T>(reinterpret_cast<const T*>(a.G)[m * a.ldg + c]);
+    dg += g * (to_f<T>(reinterpret_cast<const T*>(a.X)[m * a.ldx + c]) - a.mean[m]) * a.rstd[m];
+    db += g;
+  }
+  float* out = a.part + (size_t)blockIdx.y * 2 * a.C;
+  out[c] = dg; out[a.C + c] = db;
+}
+
+// dgamma / dbeta (+)= the P partial rows, in order: 64 columns a workgroup, its four waves take a quarter of the rows each
+__global__ __launch_bounds__(256) void ln_join_kernel(const float* part, int P, int C, float* dgamma, float* dbeta, int accumulate) {
+  __shared__ float red[4][64];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const long long n = 2ll * C, c = (long long)blockIdx.x * 64 + l;
+  float v = 0.f;
+  if (c < n) {
+    const int per = (P + 3) >> 2, p1 = (w + 1) * per < P ? (w + 1) * per : P;
+    for (int p = w * per; p < p1; ++p) v += part[p * n + c];
+  }
+  red[w][l] = v;
+  __syncthreads();
+  if (w == 0 && c < n) {
+    v = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    float* dst = c < C ? dgamma : dbeta;
+    const int cc = (int)(c < C ? c : c - C);
+    if (dst) dst[cc] = (accumulate ? dst[cc] : 0.f) + v;
+  }
+}
+
+struct LnShape { int tpr, nv; };
+// the narrowest group that holds a row in 32 elements a thread
+inline LnShape ln_shape(int C) {
+  if (C <= 128) return {16, 1};
+  if (C <= 256) return {16, 2};
+  if (C <= 512) return {64, 1};
+  if (C <= 1024) return {64, 2};
+  if (C <= 2048) return {64, 4};
+  if (C <= 4096) return {256, 2};
+  return {256, 4};
+}
+inline int ln_bwd_parts(long long M, int C) {
+  if (C > LN_REG_MAX) return (int)(M < 64 ? (M > 0 ? M : 1) : 64);
+  const long long wgs = (M + 256 / ln_shape(C).tpr - 1) / (256 / ln_shape(C).tpr);
+  return (int)(wgs < LN_BWD_WGS ? (wgs > 0 ? wgs : 1) : LN_BWD_WGS);
+}
+inline bool aligned16(const void* p, long long ld, int es) { return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0; }
+
+template <typename T, bool VEC> void launch_fwd(const spb_layernorm_args_t& a, hipStream_t s) {
+  const LnShape sh = ln_shape(a.C);
+  const long long gr = 256 / sh.tpr, need = (a.M + gr - 1) / gr;
+  const dim3 grid((unsigned)(need < LN_FWD_WGS ? need : LN_FWD_WGS)), block(256);
+#define LN_F(TPR, NV) hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, VEC>), grid, block, 0, s, a)
+  if (sh.tpr == 16) { if (sh.nv == 1) LN_F(16, 1); else LN_F(16, 2); }
+  else if (sh.tpr == 64) { if (sh.nv == 1) LN_F(64, 1); else if (sh.nv == 2) LN_F(64, 2); else LN_F(64, 4); }
+  else { if (sh.nv == 2) LN_F(256, 2); else LN_F(256, 4); }
+#undef LN_F
+}
+template <typename T, bool VEC, bool SUMS> void launch_bwd(const spb_layernorm_args_t& a, hipStream_t s) {
+  const LnShape sh = ln_shape(a.C);
+  const dim3 grid((unsigned)ln_bwd_parts(a.M, a.C)), block(256);
+#define LN_B(TPR, NV) hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV, VEC, SUMS>), grid, block, 0, s, a)
+  if (sh.tpr == 16) { if (sh.nv == 1) LN_B(16, 1); else LN_B(16, 2); }
+  else if (sh.tpr == 64) { if (sh.nv == 1) LN_B(64, 1); else if (sh.nv == 2) LN_B(64, 2); else LN_B(64, 4); }
+  else { if (sh.nv == 2) LN_B(256, 2); else LN_B(256, 4); }
+#undef LN_B
+}
+
+int check_args(int dtype, const spb_layernorm_args_t* a, bool bwd) {
+  if (dtype != SPB_F32 && dtype != SPB_BF16) return SPB_E_ARG;
+  if (!a || a->C < 1 || a->M < 0) return a ? SPB_E_SHAPE : SPB_E_ARG;
+  if (a->M == 0) return 0;
+  if (!a->X || !a->Y || !a->mean || !a->rstd || (bwd && !a->G)) return SPB_E_ARG;
+  if (a->ldx < 0 || a->ldy < (a->M > 1 ? a->C : 0) || (bwd && a->ldg < 0)) return SPB_E_SHAPE;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int spb_layernorm_fwd(int dtype, const spb_layernorm_args_t* a, spb_stream_t stream) {
+  const int bad = check_args(dtype, a, false);
+  if (bad) return bad;
+  if (a->M == 0) return 0;
+  hipStream_t s = (hipStream_t)stream;
+  const int es = dtype == SPB_F32 ? 4 : 2;
+  const bool vec = a->C % 8 == 0 && aligned16(a->X, a->ldx, es) && aligned16(a->Y, a->ldy, es);
+  if (a->C > LN_REG_MAX) {
+    const dim3 grid((unsigned)(a->M < LN_FWD_WGS ? a->M : LN_FWD_WGS));
+    if (dtype == SPB_F32) hipLaunchKernelGGL((ln_fwd_long<float>), grid, dim3(256), 0, s, *a);
+    else hipLaunchKernelGGL((ln_fwd_long<bf16_t>), grid, dim3(256), 0, s, *a);
+  } else if (dtype == SPB_F32) {
+    if (vec) launch_fwd<float, true>(*a, s); else launch_fwd<float, false>(*a, s);
+  } else {
+    if (vec) launch_fwd<bf16_t, true>(*a, s); else launch_fwd<bf16_t, false>(*a, s);
+  }
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" long long spb_layernorm_bwd_floats(long long M, int C) {
+  if (M < 0 || C < 1) return SPB_E_SHAPE;
+  return 2ll * C * ln_bwd_parts(M, C);
+}
+
+extern "C" int spb_layernorm_bwd(int dtype, const spb_layernorm_args_t* a, spb_stream_t stream) {
+  const int bad = check_args(dtype, a, true);
+  if (bad) return bad;
+  const bool sums = a->dgamma || a->dbeta;
+  if (a->M == 0 && (!sums || a->accumulate)) return 0;
+  if (sums && a->M > 0 && (!a->part || a->part_cap < spb_layernorm_bwd_floats(a->M, a->C))) return SPB_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  const int es = dtype == SPB_F32 ? 4 : 2;
+  const bool vec = a->C % 8 == 0 && aligned16(a->X, a->ldx, es) && aligned16(a->G, a->ldg, es) && aligned16(a->Y, a->ldy, es);
+  int P = ln_bwd_parts(a->M, a->C);
+  if (a->M == 0) {
+    P = 0;                                          // no rows: the join writes zeros
+  } else if (a->C > LN_REG_MAX) {
+    const long long rows = (a->M + P - 1) / P;
+    P = (int)((a->M + rows - 1) / rows);            // ranges that hold a row
+    const dim3 cols((unsigned)((a->C + 255) / 256), (unsigned)P), grid((unsigned)(a->M < LN_FWD_WGS ? a->M : LN_FWD_WGS));
+    if (dtype == SPB_F32) {
+      if (sums) hipLaunchKernelGGL((ln_bwd_cols<float>), cols, dim3(256), 0, s, *a, rows);
+      hipLaunchKernelGGL((ln_bwd_long<float>), grid, dim3(256), 0, s, *a);
+    } else {
+      if (sums) hipLaunchKernelGGL((ln_bwd_cols<bf16_t>), cols, dim3(256), 0, s, *a, rows);
+      hipLaunchKernelGGL((ln_bwd_long<bf16_t>), grid, dim3(256), 0, s, *a);
+    }
+  } else if (dtype == SPB_F32) {
+    if (sums) { if (vec) launch_bwd<float, true, true>(*a, s); else launch_bwd<float, false, true>(*a, s); }
+    else { if (vec) launch_bwd<float, true, false>(*a, s); else launch_bwd<float, false, false>(*a, s); }
+  } else {
+    if (sums) { if (vec) launch_bwd<bf16_t, true, true>(*a, s); else launch_bwd<bf16_t, false, true>(*a, s); }
+    else { if (vec) launch_bwd<bf16_t, true, false>(*a, s); else launch_bwd<bf16_t, false, false>(*a, s); }
+  }
+  SPB_CHECK_LAUNCH();
+  if (sums) {
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((2ll * a->C + 63) / 64)), dim3(256), 0, s, a->part, P, a->C, a->dgamma, a->dbeta, a->accumulate);
+    SPB_CHECK_LAUNCH();
+  }
+  return 0;
+}

@@ -1,0 +1,284 @@
+// Packing to 8 bits with one power-of-two scale for each block of 128 (format: include/spb_hip.h "8-bit packing"), and the activations that keep
+// their input in that form for the backward pass.
+//
+//   block top a = max |x| over its finite elements,  e = smallest integer with a <= 448 * 2^e,  code = e4m3(x * 2^-e)
+//   act8 forward  y = act(x), checkpoint = pack(x);    backward  dx = g * act'(value(checkpoint))
+//
+// The scale is a power of two so that packing has ONE rounding (the code's own), its result does not depend on how a quotient is rounded, values
+// stay exact in bfloat16, and the matrix instructions apply it themselves.  It costs at most one bit of exponent range, which e4m3 has to spare.
+// All of it is bound by HBM: every element is read once and written once.  16 lanes share a block of 128 (8 consecutive elements each: 16-byte
+// loads of 16-bit types, 8-byte stores of codes), its top is four vector-ALU exchanges, and neighbouring groups hold neighbouring blocks.
+#include "pack8.h"
+
+namespace {
+
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, spb_dpp_f<0xB1>(v)); v = fmaxf(v, spb_dpp_f<0x4E>(v)); v = fmaxf(v, spb_dpp_f<0x141>(v)); v = fmaxf(v, spb_dpp_f<0x140>(v));
+  return v;
+}
+// 8 elements from column c on (zeros behind K).  VEC: 16-byte aligned rows and K % 8 == 0.
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, int c, int K, float v[8]) {
+  if (VEC) {
+    float t[8];
+    ld8<T>(row + (c < K ? c : 0), t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c < K ? t[i] : 0.f;
+  } else {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = row[c + i < K ? c + i : 0];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f<T>(t[i]) : 0.f;
+  }
+}
+// The f32 value is what is rounded, in both forms: without the empty asm the compiler may fold a product into its conversion to half (one rounding
+// instead of two) in one of them, and a result would depend on its tensor's alignment.
+template <typename T, bool VEC> __device__ __forceinline__ void store8(T* row, int c, int K, float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) asm("" : "+v"(v[i]));
+  if (VEC) {
+    if (c < K) st8<T>(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < K) row[c + i] = from_f<T>(v[i]);
+  }
+}
+
+// act'(x) and act(x) in f32.  ACT 0: none (plain packing).
+template <int ACT> __device__ __forceinline__ float act8(float x) {
+  if (ACT == SPB_ACT_SILU) return x / (1.f + expf(-x));
+  if (ACT == SPB_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
+  if (ACT == SPB_ACT_GELU_TANH) return 0.5f * x * (1.f + tanhf(0.79788456f * (x + 0.044715f * x * x * x)));
+  return x;
+}
+template <int ACT> __device__ __forceinline__ float act8_slope(float x) {
+  if (ACT == SPB_ACT_SILU) { const float s = 1.f / (1.f + expf(-x)); return s * (1.f + x * (1.f - s)); }
+  if (ACT == SPB_ACT_GELU) return 0.5f * (1.f + erff(x * 0.70710678f)) + x * 0.39894228f * expf(-0.5f * x * x);
+  x = x > 16.f ? 16.f : (x < -16.f ? -16.f : x);       // 1 - t^2 is 0 from there on; x * x would overflow in 0 * inf.  NaN stays NaN.
+  const float t = tanhf(0.79788456f * (x + 0.044715f * x * x * x));
+  return 0.5f * (1.f + t) + 0.5f * x * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * x * x);
+}
+
+struct RowArgs {
+  const void* X; void* Y; unsigned char* Q; unsigned char* S;
+  long long ldx, ldy;
+  unsigned blocks;      // M * KB
+  int K, KB, Kp, Sp;
+};
+template <typename T, bool VEC, int ACT>
+__global__ __launch_bounds__(256) void pack8_rows_kernel(const RowArgs a) {
+  const unsigned u = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int l = threadIdx.x & 15;
+  if (u >= a.blocks) return;                           // whole groups of 16 lanes: the exchanges below stay inside a group
+  const unsigned m = u / (unsigned)a.KB;
+  const int kb = (int)(u - m * (unsigned)a.KB), c = kb * P8_BLOCK + l * 8;
+  float v[8];
+  load8<T, VEC>(reinterpret_cast<const T*>(a.X) + (long long)m * a.ldx, c, a.K, v);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, p8_finite_abs(v[i]));
+  const int e = p8_exponent(row16_max(top));
+  *reinterpret_cast<uint2*>(a.Q + (size_t)m * a.Kp + c) = p8_encode8(v, e);
+  unsigned char* s = a.S + (size_t)m * a.Sp;
+  if (l == 0) s[kb] = (unsigned char)(e + 127);
+  else if (kb == a.KB - 1 && a.KB - 1 + l < a.Sp) s[a.KB - 1 + l] = 127;
+  if (ACT != 0) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = act8<ACT>(v[i]);
+    store8<T, VEC>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, y);
+  }
+}
+
+// values of a packed matrix (ACT 0) or g * act'(value): a thread 8 elements
+struct UnpackArgs {
+  const void* G; void* Y; const unsigned char* Q; const unsigned char* S;
+  long long ldg, ldy;
+  unsigned vecs;        // M * V
+  int K, V, Kp, Sp, shift;
+};
+template <typename T, bool VEC, int ACT>
+__global__ __launch_bounds__(256) void unpack8_kernel(const UnpackArgs a) {
+  const unsigned u = blockIdx.x * 256 + threadIdx.x;
+  if (u >= a.vecs) return;
+  const unsigned m = u / (unsigned)a.V;
+  const int c = (int)(u - m * (unsigned)a.V) * 8;
+  const uint2 q = *reinterpret_cast<const uint2*>(a.Q + (size_t)m * a.Kp + c);
+  const float s = p8_pow2((int)a.S[(size_t)(m >> a.shift) * a.Sp + (c >> 7)] - 127);
+  float v[8];
+  p8_decode8(q, s, v);
+  if (ACT != 0) {
+    float g[8];
+    load8<T, VEC>(reinterpret_cast<const T*>(a.G) + (long long)m * a.ldg, c, a.K, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = g[i] * act8_slope<ACT>(v[i]);
+  }
+  store8<T, VEC>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, v);
+}
+
+// a 128 x 128 block a workgroup: 16 lanes hold 128 columns of a row, 16 rows at a time.  The transposed codes go through LDS (rows of 144 bytes:
+// 16-byte reads, and the 4-byte bank of a byte column moves with its row).
+struct WeightArgs {
+  const void* W; unsigned char* Q; unsigned char* S; unsigned char* QT; unsigned char* ST;
+  long long ldw;
+  int N, K, NB, KB, Kp, Sp, Np, SpT;
+};
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void pack8_weight_kernel(const WeightArgs a) {
+  constexpr int LD = 144;
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) unsigned char tile[128 * LD];     // [column][row]
+  const int nb = blockIdx.x / a.KB, kb = blockIdx.x - nb * a.KB;
+  const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = kb * P8_BLOCK + l * 8;
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = nb * P8_BLOCK + r0 + 16 * i;
+    load8<T, VEC>(reinterpret_cast<const T*>(a.W) + (long long)(n < a.N ? n : 0) * a.ldw, c, a.K, v[i]);
+    if (n >= a.N) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, p8_finite_abs(v[i][j]));
+  top = row16_max(top);
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  const int e = p8_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i, n = nb * P8_BLOCK + r;
+    const uint2 q = p8_encode8(v[i], e);
+    if (n < a.N) *reinterpret_cast<uint2*>(a.Q + (size_t)n * a.Kp + c) = q;
+    if (a.QT) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) tile[(l * 8 + j) * LD + r] = (unsigned char)((j < 4 ? q.x >> (8 * j) : q.y >> (8 * (j - 4))) & 255u);
+    }
+  }
+  if (threadIdx.x == 0) a.S[(size_t)nb * a.Sp + kb] = (unsigned char)(e + 127);
+  else if (kb == a.KB - 1 && kb + (int)threadIdx.x < a.Sp) a.S[(size_t)nb * a.Sp + kb + threadIdx.x] = 127;
+  if (a.QT) {
+    if (threadIdx.x == 0) a.ST[(size_t)kb * a.SpT + nb] = (unsigned char)(e + 127);
+    else if (nb == a.NB - 1 && nb + (int)threadIdx.x < a.SpT) a.ST[(size_t)kb * a.SpT + nb + threadIdx.x] = 127;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int idx = threadIdx.x + 256 * i, col = idx >> 3, part = idx & 7, k = kb * P8_BLOCK + col;
+      if (k < a.K)
+        *reinterpret_cast<uint4*>(a.QT + (size_t)k * a.Np + nb * P8_BLOCK + part * 16) = *reinterpret_cast<const uint4*>(tile + col * LD + part * 16);
+    }
+  }
+}
+
+inline bool rows_aligned(const void* p, long long ld, int es, int K) { return K % 8 == 0 && ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0; }
+inline bool bad_codes(const void* q, const void* s) { return !q || !s || ((uintptr_t)q & 15) || ((uintptr_t)s & 3); }
+inline bool bad_dtype(int d) { return d != SPB_F32 && d != SPB_BF16; }
+
+template <int ACT> int pack_rows(int dtype, RowArgs a, long long M, hipStream_t s) {
+  const int es = dtype == SPB_F32 ? 4 : 2;
+  bool vec = rows_aligned(a.X, a.ldx, es, a.K);
+  if (ACT != 0) vec = vec && rows_aligned(a.Y, a.ldy, es, a.K);
+  if (M * a.KB > 0xfffffff0ll) return SPB_E_SHAPE;
+  a.blocks = (unsigned)(M * a.KB);
+  const dim3 grid(a.blocks / 16 + (a.blocks % 16 ? 1 : 0));
+  if (dtype == SPB_F32) {
+    if (vec) hipLaunchKernelGGL((pack8_rows_kernel<float, true, ACT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((pack8_rows_kernel<float, false, ACT>), grid, dim3(256), 0, s, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((pack8_rows_kernel<bf16_t, true, ACT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((pack8_rows_kernel<bf16_t, false, ACT>), grid, dim3(256), 0, s, a);
+  }
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+template <int ACT> int unpack(int dtype, UnpackArgs a, long long M, hipStream_t s) {
+  const int es = dtype == SPB_F32 ? 4 : 2;
+  bool vec = rows_aligned(a.Y, a.ldy, es, a.K);
+  if (ACT != 0) vec = vec && rows_aligned(a.G, a.ldg, es, a.K);
+  if (M * a.V > 0xfffffff0ll) return SPB_E_SHAPE;
+  a.vecs = (unsigned)(M * a.V);
+  const dim3 grid(a.vecs / 256 + (a.vecs % 256 ? 1 : 0));
+  if (dtype == SPB_F32) {
+    if (vec) hipLaunchKernelGGL((unpack8_kernel<float, true, ACT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((unpack8_kernel<float, false, ACT>), grid, dim3(256), 0, s, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((unpack8_kernel<bf16_t, true, ACT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((unpack8_kernel<bf16_t, false, ACT>), grid, dim3(256), 0, s, a);
+  }
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int spb_pack8_rows(int dtype, const void* X, long long ldx, long long M, int K, unsigned char* codes, unsigned char* scales, spb_stream_t stream) {
+  if (bad_dtype(dtype)) return SPB_E_ARG;
+  if (M < 0 || K < 0 || ldx < 0) return SPB_E_SHAPE;
+  if (M == 0 || K == 0) return 0;
+  if (!X || bad_codes(codes, scales)) return SPB_E_ARG;
+  return pack_rows<0>(dtype, {X, nullptr, codes, scales, ldx, 0, 0, K, (K + 127) / 128, p8_cols(K), p8_scales(K)}, M, (hipStream_t)stream);
+}
+
+extern "C" int spb_pack8_weight(int dtype, const void* W, long long ldw, int N, int K, unsigned char* codes, unsigned char* scales, unsigned char* codesT,
+                                unsigned char* scalesT, spb_stream_t stream) {
+  if (bad_dtype(dtype)) return SPB_E_ARG;
+  if (N < 0 || K < 0 || ldw < 0) return SPB_E_SHAPE;
+  if (N == 0 || K == 0) return 0;
+  if (!W || bad_codes(codes, scales) || (codesT != nullptr) != (scalesT != nullptr) || (codesT && bad_codes(codesT, scalesT))) return SPB_E_ARG;
+  const WeightArgs a = {W, codes, scales, codesT, scalesT, ldw, N, K, (N + 127) / 128, (K + 127) / 128, p8_cols(K), p8_scales(K), p8_cols(N), p8_scales(N)};
+  if ((long long)a.NB * a.KB > 0x7fffffffll) return SPB_E_SHAPE;
+  const bool vec = rows_aligned(W, ldw, dtype == SPB_F32 ? 4 : 2, K);
+  const dim3 grid((unsigned)(a.NB * a.KB));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == SPB_F32) {
+    if (vec) hipLaunchKernelGGL((pack8_weight_kernel<float, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((pack8_weight_kernel<float, false>), grid, dim3(256), 0, s, a);
+  } else {
+    if (vec) hipLaunchKernelGGL((pack8_weight_kernel<bf16_t, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((pack8_weight_kernel<bf16_t, false>), grid, dim3(256), 0, s, a);
+  }
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+
+extern "C" int spb_unpack8(int dtype, const unsigned char* codes, const unsigned char* scales, int block_rows, long long M, int K, void* Y, long long ldy,
+                           spb_stream_t stream) {
+  if (bad_dtype(dtype) || (block_rows != 1 && block_rows != 128)) return SPB_E_ARG;
+  if (M < 0 || K < 0 || (M > 1 && ldy < K)) return SPB_E_SHAPE;
+  if (M == 0 || K == 0) return 0;
+  if (!Y || bad_codes(codes, scales)) return SPB_E_ARG;
+  return unpack<0>(dtype, {nullptr, Y, codes, scales, 0, ldy, 0, K, (K + 7) / 8, p8_cols(K), p8_scales(K), block_rows == 128 ? 7 : 0}, M, (hipStream_t)stream);
+}
+
+extern "C" int spb_act8_fwd(int dtype, int act, const void* X, long long ldx, void* Y, long long ldy, long long M, int K, unsigned char* codes,
+                            unsigned char* scales, spb_stream_t stream) {
+  if (bad_dtype(dtype) || act < SPB_ACT_GELU || act > SPB_ACT_SILU) return SPB_E_ARG;
+  if (M < 0 || K < 0 || ldx < 0 || (M > 1 && ldy < K)) return SPB_E_SHAPE;
+  if (M == 0 || K == 0) return 0;
+  if (!X || !Y || bad_codes(codes, scales)) return SPB_E_ARG;
+  const RowArgs a = {X, Y, codes, scales, ldx, ldy, 0, K, (K + 127) / 128, p8_cols(K), p8_scales(K)};
+  hipStream_t s = (hipStream_t)stream;
+  if (act == SPB_ACT_GELU) return pack_rows<SPB_ACT_GELU>(dtype, a, M, s);
+  if (act == SPB_ACT_GELU_TANH) return pack_rows<SPB_ACT_GELU_TANH>(dtype, a, M, s);
+  return pack_rows<SPB_ACT_SILU>(dtype, a, M, s);
+}
+
+extern "C" int spb_act8_bwd(int dtype, int act, const void* G, long long ldg, const unsigned char* codes, const unsigned char* scales, void* dX,
+                            long long ldd, long long M, int K, spb_stream_t stream) {
+  if (bad_dtype(dtype) || act < SPB_ACT_GELU || act > SPB_ACT_SILU) return SPB_E_ARG;
+  if (M < 0 || K < 0 || ldg < 0 || (M > 1 && ldd < K)) return SPB_E_SHAPE;
+  if (M == 0 || K == 0) return 0;
+  if (!G || !dX || bad_codes(codes, scales)) return SPB_E_ARG;
+  const UnpackArgs a = {G, dX, codes, scales, ldg, ldd, 0, K, (K + 7) / 8, p8_cols(K), p8_scales(K), 0};
+  hipStream_t s = (hipStream_t)stream;
+  if (act == SPB_ACT_GELU) return unpack<SPB_ACT_GELU>(dtype, a, M, s);
+  if (act == SPB_ACT_GELU_TANH) return unpack<SPB_ACT_GELU_TANH>(dtype, a, M, s);
+  return unpack<SPB_ACT_SILU>(dtype, a, M, s);
+}

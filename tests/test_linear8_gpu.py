@@ -1,0 +1,449 @@
+"""8-bit packing, the product of packed operands, the weight gradient from an 8-bit checkpoint and the activations that keep one (csrc/pack8.hip,
+gemm8.hip, wgrad8.hip) against their definitions in float64.
+
+Packing has one rounding, the code's own: it is compared for equality.  u = 2^-24, h = torch.finfo(t).eps / 2 of the output's type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def place(x, layout):
+    M, C = x.shape
+    if layout == "dense":
+        return x.cuda()
+    if layout == "slab":
+        w = torch.full((M, (C + 7) // 8 * 8 + 16), float("nan"), dtype=x.dtype)
+        w[:, 8:8 + C] = x
+        return w.cuda()[:, 8:8 + C]
+    w = torch.full((M * C + 3,), float("nan"), dtype=x.dtype)
+    w[3:] = x.reshape(-1)
+    return w.cuda()[3:].view(M, C)
+
+
+def data(M, K, dtype, seed, layout="dense", scale=1.0):
+    """rows and columns of different size, some exact zeros"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g) * torch.exp2(torch.randint(-6, 7, (M, 1), generator=g).float()) * torch.exp2(torch.randint(-3, 4, (1, K), generator=g).float())
+    x[torch.rand(M, K, generator=g) < 0.05] = 0
+    return place((x * scale).to(dtype), layout)
+
+
+def exponents(x, rows):
+    """exponent of every rows x 128 block of x (float64, CPU): the smallest e with max |finite x| <= 448 * 2^e, in [-110, 120]; 0 without any"""
+    M, K = x.shape
+    mb, kb = -(-M // rows), -(-K // 128)
+    p = torch.zeros(mb * rows, kb * 128, dtype=torch.float64)
+    p[:M, :K] = torch.where(x.isfinite(), x, torch.zeros_like(x)).abs()
+    top = p.view(mb, rows, kb, 128).amax((1, 3))
+    e = torch.full_like(top, -110.0)
+    for k in range(-110, 120):
+        e[top > 448 * 2.0 ** k] = k + 1
+    e[top == 0] = 0
+    return e.to(torch.int64)
+
+
+def codes_of(x, e, rows):
+    """the codes (uint8 as int64) by comparing with all 127 magnitudes: nearest, ties to the even code"""
+    M, K = x.shape
+    s = (2.0 ** e.double()).repeat_interleave(rows, 0).repeat_interleave(128, 1)[:M, :K]
+    mags = torch.arange(127).to(torch.uint8).view(torch.float8_e4m3fn).double()
+    mid = (mags[1:] + mags[:-1]) / 2
+    a = (x / s).abs()
+    c = torch.searchsorted(mid, a.contiguous(), right=False)         # midpoints go down ...
+    tie = (c < 126) & (a == mid[c.clamp(max=125)])
+    c = c + (tie & (c % 2 == 1))                                      # ... unless the code below is odd
+    c = torch.where((s == 2.0 ** 120) & (c * 1 > 119), torch.full_like(c, 119), c)     # 256 * 2^120 is no float: the code of 240
+    c = torch.where(x.isfinite(), c, torch.full_like(c, 127))
+    sign = torch.signbit(x).to(torch.int64) * 128
+    return c, sign
+
+
+def same_codes(got, c, sign):
+    got = got.cpu().to(torch.int64)
+    return torch.equal(got & 127, c) and torch.equal(torch.where(c == 127, sign, got & 128), sign)
+
+
+SPECIAL = [0.0, -0.0, 448.0, 449.0, -1.0, 1.0625, 1.1875, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -11, 0.015625, 0.0146484375, 240.0, 232.0, 248.0, 26.0, 27.0]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["dense", "slab", "odd"])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 128), (3, 127), (2, 129), (5, 8), (7, 1000), (33, 520), (2, 4104), (130, 257), (1, 9216)])
+def test_pack_rows(device, M, K, layout, dtype):
+    from speedplusbaseline_amd import ops
+    x = data(M, K, dtype, M * K, layout)
+    P = ops.quant8(x)
+    c = x.cpu().double()
+    e = exponents(c, 1)
+    kb = -(-K // 128)
+    assert P.shape == (M, K) and P.codes.shape == (M, kb * 128) and P.scales.shape == (M, (kb + 3) // 4 * 4)
+    assert torch.equal(P.scales.cpu()[:, :kb].to(torch.int64), e + 127) and (P.scales[:, kb:] == 127).all()
+    assert same_codes(P.codes[:, :K], *codes_of(c, e, 1)) and (P.codes[:, K:] == 0).all()
+    for t in TYPES:
+        v = ops.dequant8(P, t)
+        want = P.codes.cpu()[:, :K].view(torch.float8_e4m3fn).double() * (2.0 ** e.double()).repeat_interleave(128, 1)[:, :K]
+        assert v.dtype == t and torch.equal(v.cpu(), want.to(t))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["dense", "slab", "odd"])
+@pytest.mark.parametrize("N,K", [(1, 1), (128, 128), (3, 300), (129, 130), (1000, 200), (96, 1280), (257, 8)])
+def test_pack_weight(device, N, K, layout, dtype):
+    from speedplusbaseline_amd import ops
+    w = data(N, K, dtype, N + K, layout)
+    P, T = ops.quant8_weight(w)
+    c = w.cpu().double()
+    e = exponents(c, 128)
+    nb, kb = -(-N // 128), -(-K // 128)
+    assert P.scales.shape == (nb, (kb + 3) // 4 * 4) and T.scales.shape == (kb, (nb + 3) // 4 * 4)
+    assert torch.equal(P.scales.cpu()[:, :kb].to(torch.int64), e + 127) and (P.scales[:, kb:] == 127).all()
+    assert torch.equal(T.scales.cpu()[:, :nb].to(torch.int64), e.t() + 127) and (T.scales[:, nb:] == 127).all()
+    assert same_codes(P.codes[:, :K], *codes_of(c, e, 128)) and (P.codes[:, K:] == 0).all()
+    assert torch.equal(T.codes[:, :N], P.codes[:, :K].t()) and (T.codes[:, N:] == 0).all()
+    assert torch.equal(ops.dequant8(T, torch.float32).t(), ops.dequant8(P, torch.float32))
+    Q, none = ops.quant8_weight(w, transpose=False)
+    assert none is None and torch.equal(Q.codes, P.codes)
+
+
+def test_pack_special_values(device):
+    from speedplusbaseline_amd import ops
+    big = torch.finfo(torch.float32).max
+    rows = [SPECIAL, [v * 2.0 ** 100 for v in SPECIAL], [v * 2.0 ** -100 for v in SPECIAL], [v * 2.0 ** -139 for v in SPECIAL],
+            [big, -big, 1.9 * 2.0 ** 127, 1.95 * 2.0 ** 127, 2.0 ** 120, 2.0 ** 108], [0.0] * 4, [float("inf"), 1.0, -2.0, float("nan"), -float("inf")],
+            [float("nan")] * 3, [448 * 2.0 ** 5, 1.0], [torch.nextafter(torch.tensor(448 * 2.0 ** 5), torch.tensor(1e9)).item(), 1.0], [2.0 ** -149, 0.0]]
+    # ties of every code, with 448 in the block so that the exponent is 0
+    m = torch.arange(127).to(torch.uint8).view(torch.float8_e4m3fn).float()
+    mids = (m[1:] + m[:-1]) / 2
+    rows += [[448.0] + mids.tolist(), [448.0] + torch.nextafter(mids, torch.tensor(0.0)).tolist(), [448.0] + torch.nextafter(mids, torch.tensor(1e9)).tolist()]
+    x = torch.zeros(len(rows), 128)
+    for i, r in enumerate(rows):
+        x[i, :len(r)] = torch.tensor(r)
+    P = ops.quant8(x.cuda())
+    c = x.double()
+    e = exponents(c, 1)
+    assert torch.equal(P.scales.cpu()[:, :1].to(torch.int64), e + 127)
+    assert same_codes(P.codes, *codes_of(c, e, 1))
+    v = ops.dequant8(P, torch.float32).cpu()
+    assert torch.equal(v.isfinite(), x.isfinite()) and torch.equal(ops.dequant8(P, torch.bfloat16).cpu().float()[v.isfinite()], v[v.isfinite()])
+    # packing the values again gives the same codes
+    again = ops.quant8(v.cuda())
+    ok = x.isfinite().all(1) & (v.abs().amax(1) > 0)
+    assert torch.equal(ops.dequant8(again, torch.float32).cpu()[ok], v[ok])
+
+
+# ---- product ----------------------------------------------------------------------------------------------------------------------------------
+def values(P):
+    from speedplusbaseline_amd import ops
+    return ops.dequant8(P, torch.float32).double()
+
+
+def check_product(A, B, bias, y):
+    """float32 output: exact products, K / 8 accumulations of at most 8 products each are rounded (every partial sum is at most the sum of magnitudes).
+    16-bit output: the 8-bit instruction aligns 8 neighbouring products to the largest of them and drops what is below 2^-13 of its power of two
+    (1 and -1 beside 2^-13: kept, beside 2^-14: lost; products 8 places apart keep 24 bits; measured lane by lane).  The largest product itself has 8 bits
+    and is whole, the other seven lose less than 2^-13 of it each: at most 7 * 2^-13 * max|a| * max|b| for 8 neighbours, added up over the row."""
+    a, b = values(A), values(B)
+    ref, mag = a @ b.t(), a.abs() @ b.abs().t()
+    if bias is not None:
+        ref, mag = ref + bias.double(), mag + bias.double().abs()
+    K = A.K
+    lim = (K / 8 + 8) * U * mag
+    if y.dtype != torch.float32:
+        top = lambda v: torch.nn.functional.pad(v.abs(), (0, -K % 8)).view(v.shape[0], -1, 8).amax(2)          # noqa: E731
+        lim = lim + 7 * 2.0 ** -13 * (top(a) @ top(b).t())
+    lim = lim * (1 + half(y.dtype)) + half(y.dtype) * ref.abs() + 2.0 ** -24 * (y.dtype == torch.float16) + 1e-40
+    assert y.shape == ref.shape
+    assert ((y.double() - ref).abs() <= lim).all(), ((y.double() - ref).abs() / lim).max()
+
+
+PRODUCTS = [(1, 1, 1), (1, 8, 128), (1, 4096, 1024), (2, 17, 129), (3, 130, 640), (15, 64, 300), (16, 16, 128), (17, 33, 127), (48, 1000, 2304), (63, 200, 513),
+            (64, 256, 256), (65, 70, 1000), (100, 128, 8), (128, 128, 512), (129, 257, 1001), (200, 300, 4104), (257, 129, 130), (500, 640, 1152), (1000, 96, 64)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_product(device, M, N, K, dtype):
+    from speedplusbaseline_amd import ops
+    x, w = data(M, K, torch.bfloat16, M, scale=0.02), data(N, K, torch.float32, N, scale=0.02)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(2)).cuda()
+    A, (B, _) = ops.quant8(x), ops.quant8_weight(w)
+    check_product(A, B, bias, ops.gemm8(A, B, bias=bias, dtype=dtype))
+    R = ops.quant8(w)                            # scales by rows on both sides
+    check_product(A, R, None, ops.gemm8(A, R, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(1, 40, 256), (5, 17, 1024), (48, 264, 640), (300, 1500, 512), (1024, 1152, 384)])
+def test_product_of_whole_numbers_is_exact(device, M, N, K, dtype):
+    """codes -4 .. 4 (scales set by a 448 in a column the other side has 0 in): every sum is a whole number below 2^24, in any order"""
+    from speedplusbaseline_amd import ops
+    g = torch.Generator().manual_seed(K)
+    x, w = torch.randint(-4, 5, (M, K), generator=g).float(), torch.randint(-4, 5, (N, K), generator=g).float()
+    x[:, 0::128] = 448; w[:, 0::128] = 0
+    w[:, 1::128] = 448; x[:, 1::128] = 0
+    y = ops.gemm8(ops.quant8(x.cuda()), ops.quant8_weight(w.cuda())[0], dtype=dtype)
+    assert torch.equal(y.cpu(), (x.double() @ w.double().t()).to(dtype))
+
+
+def test_product_into_a_slab_and_with_nothing_to_add(device):
+    from speedplusbaseline_amd import ops
+    for dtype in TYPES:
+        A, (B, _) = ops.quant8(data(37, 200, dtype, 1)), ops.quant8_weight(data(50, 200, dtype, 2))
+        want = ops.gemm8(A, B, dtype=dtype)
+        for off, width in ((8, 72), (3, 59)):
+            wide = torch.full((37, width), 7.0, dtype=dtype, device="cuda")
+            y = ops.gemm8(A, B, dtype=dtype, Y=wide[:, off:off + 50])
+            assert torch.equal(y, want) and (wide[:, :off] == 7).all() and (wide[:, off + 50:] == 7).all()
+        bias = torch.randn(50, device="cuda")
+        E, (F, _) = ops.quant8(torch.empty(37, 0, dtype=dtype, device="cuda")), ops.quant8_weight(torch.empty(50, 0, dtype=dtype, device="cuda"))
+        assert torch.equal(ops.gemm8(E, F, bias=bias, dtype=dtype), bias.to(dtype).expand(37, 50))
+        assert ops.gemm8(ops.quant8(torch.empty(0, 200, dtype=dtype, device="cuda")), B, dtype=dtype).shape == (0, 50)
+        assert ops.gemm8(A, ops.quant8(torch.empty(0, 200, dtype=dtype, device="cuda")), dtype=dtype).shape == (37, 0)
+
+
+def test_nonfinite_elements_spoil_their_rows_only(device):
+    from speedplusbaseline_amd import ops
+    x, w = data(70, 300, torch.float32, 1), data(140, 300, torch.float32, 2)
+    clean = {t: ops.gemm8(ops.quant8(x), ops.quant8_weight(w)[0], dtype=t) for t in TYPES}
+    x2 = x.clone()
+    x2[5, 17], x2[69, 299] = float("inf"), float("nan")
+    for t in TYPES:
+        y = ops.gemm8(ops.quant8(x2), ops.quant8_weight(w)[0], dtype=t)
+        keep = [i for i in range(70) if i not in (5, 69)]
+        assert torch.isnan(y[[5, 69]]).all() and torch.equal(y[keep], clean[t][keep])
+
+
+def test_codes_behind_two_to_the_32(device):
+    """A's codes take 5.2 GB; the rows at their end are those of a small product"""
+    from speedplusbaseline_amd import ops
+    M, K, N = 20000, 262144, 24
+    P = ops.Packed8.empty(M, K, 1, torch.device("cuda:0"))
+    P.codes.zero_(); P.scales.fill_(127)
+    tail, w = data(3, K, torch.bfloat16, 1, scale=0.01), data(N, K, torch.bfloat16, 2, scale=0.01)
+    t8, (w8, _) = ops.quant8(tail), ops.quant8_weight(w, transpose=False)
+    P.codes[-3:] = t8.codes; P.scales[-3:] = t8.scales
+    y = ops.gemm8(P, w8, dtype=torch.float32)
+    assert (y[:-3] == 0).all()
+    check_product(t8, w8, None, y[-3:])
+    g = torch.zeros(M, 8, device="cuda"); g[-3:] = data(3, 8, torch.float32, 4)
+    check_wgrad(g[-3:], t8, ops.gemm8_wgrad(g, P))
+
+
+# ---- weight gradient ---------------------------------------------------------------------------------------------------------------------------
+def check_wgrad(G, X8, dw, before=None):
+    """every product is exact; M / 8 accumulations (each piece of a gradient that is split has its own), 64 partial sums at most"""
+    x, g = values(X8), G.double()
+    ref, mag = g.t() @ x, g.abs().t() @ x.abs()
+    pieces = {torch.float32: 3, torch.bfloat16: 1, torch.float16: 2}[G.dtype]
+    lim = (pieces * (G.shape[0] / 8 + 8) + 64) * U * mag + 1e-40
+    if before is not None:
+        ref = ref + before
+        lim = lim + 2 * U * ref.abs()
+    assert ((dw.double() - ref).abs() <= lim).all(), ((dw.double() - ref).abs() / lim).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["dense", "slab", "odd"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 128), (5, 17, 129), (63, 130, 64), (64, 8, 1000), (65, 256, 257), (300, 144, 24), (1000, 200, 136), (2351, 33, 640)])
+def test_wgrad(device, M, N, K, layout, dtype):
+    from speedplusbaseline_amd import ops
+    G, X8 = data(M, N, dtype, M, layout, scale=1e-3), ops.quant8(data(M, K, torch.bfloat16, N))
+    check_wgrad(G, X8, ops.gemm8_wgrad(G, X8))
+    wide = torch.randn(N, K + 5, device="cuda")
+    before = wide.double()
+    out = ops.gemm8_wgrad(G, X8, dW=wide[:, 2:2 + K])
+    check_wgrad(G, X8, out, before[:, 2:2 + K])
+    assert torch.equal(wide[:, :2].double(), before[:, :2]) and torch.equal(wide[:, 2 + K:].double(), before[:, 2 + K:])
+
+
+def test_wgrad_keeps_all_bits_of_the_gradient(device):
+    """one row: dW is the outer product, exact up to its own rounding"""
+    from speedplusbaseline_amd import ops
+    for dtype in TYPES:
+        G, x = data(1, 300, dtype, 3), torch.ones(1, 40, device="cuda")
+        G[0, :4] = torch.tensor([0.0, 2.0 ** -14 * 1.0009765625, 65504.0, -1 / 3], device="cuda").to(dtype)
+        dw = ops.gemm8_wgrad(G, ops.quant8(x))
+        assert torch.equal(dw, G.float().t().expand(300, 40))
+    G = torch.ones(3, 8, device="cuda"); G[1, 2], G[2, 5] = float("inf"), float("nan")
+    dw = ops.gemm8_wgrad(G, ops.quant8(torch.ones(3, 16, device="cuda")))
+    assert not dw[2].isfinite().any() and not dw[5].isfinite().any() and (dw[[0, 1, 3, 4, 6, 7]] == 3).all()
+
+
+def test_wgrad_without_rows(device):
+    from speedplusbaseline_amd import ops
+    G, X8 = torch.empty(0, 20, device="cuda"), ops.quant8(torch.empty(0, 30, device="cuda"))
+    assert (ops.gemm8_wgrad(G, X8) == 0).all()
+    dw = torch.ones(20, 30, device="cuda")
+    assert (ops.gemm8_wgrad(G, X8, dW=dw) == 1).all()
+
+
+# ---- activations -------------------------------------------------------------------------------------------------------------------------------
+def act_ref(x, act):
+    from speedplusbaseline_amd import _lib as L
+    F = torch.nn.functional
+    return {L.ACT_GELU: F.gelu, L.ACT_GELU_TANH: lambda v: F.gelu(v, approximate="tanh"), L.ACT_SILU: F.silu}[act](x)
+
+
+def slope_ref(x, act):
+    x = x.clone().requires_grad_()
+    g, = torch.autograd.grad(act_ref(x, act).sum(), x)
+    return g
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("act", ["ACT_GELU", "ACT_GELU_TANH", "ACT_SILU"])
+@pytest.mark.parametrize("layout", ["dense", "slab", "odd"])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 130), (9, 1280), (257, 72)])
+def test_activation_with_checkpoint(device, M, K, layout, act, dtype):
+    """y: the functions' arguments and values carry a few roundings each, on terms of at most |x|: 8 u |x|.  dx: the slopes' terms are at most 1.2 (x phi(x),
+    x s (1 - s)) and their arguments' roundings move them by |x|^3 phi(x) u at most: 32 u |g|."""
+    from speedplusbaseline_amd import _lib as L, ops
+    act = getattr(L, act)
+    x = data(M, K, dtype, K, layout, scale=0.2)
+    y, P = ops.act8_fwd(x, act)
+    ref = act_ref(x.double(), act)
+    lim = 8 * U * x.double().abs() + half(dtype) * ref.abs() + 2.0 ** -24 * (dtype == torch.float16)
+    assert ((y.double() - ref).abs() <= lim).all()
+    Q = ops.quant8(x)
+    assert torch.equal(P.codes, Q.codes) and torch.equal(P.scales, Q.scales)
+    g = data(M, K, dtype, K + 1, layout)
+    dx = ops.act8_bwd(g, P, act)
+    ref = g.double() * slope_ref(values(P), act)
+    lim = 32 * U * g.double().abs() + half(dtype) * ref.abs() + 2.0 ** -24 * (dtype == torch.float16)
+    assert dx.dtype == dtype and ((dx.double() - ref).abs() <= lim).all(), ((dx.double() - ref).abs() / lim).max()
+    dense_g = g.clone()
+    assert torch.equal(ops.act8_bwd(dense_g, P, act, dX=dense_g), dx)
+    dense_x = x.clone()
+    assert torch.equal(ops.act8_fwd(dense_x, act, Y=dense_x)[0], y)
+
+
+def test_activation_far_out_and_nonfinite(device):
+    from speedplusbaseline_amd import _lib as L, ops
+    x = torch.tensor([[0.0, -0.0, 3e38, -3e38, 1e4, -1e4, 100.0, -100.0, 20.0, -20.0, 1e-30, -1e-30, float("nan"), float("inf")]], device="cuda").t().contiguous()
+    for act in (L.ACT_GELU, L.ACT_GELU_TANH, L.ACT_SILU):
+        y, P = ops.act8_fwd(x, act)
+        dx = ops.act8_bwd(torch.ones_like(x), P, act)
+        v = values(P)
+        fin = x.isfinite()
+        ref = act_ref(x.double(), act)
+        assert ((y.double() - ref).abs()[fin] <= 8 * U * x.double().abs()[fin]).all()
+        want = torch.where(v.abs() > 15, (v > 0).double(), slope_ref(v.clamp(-15, 15), act))
+        assert ((dx.double() - want).abs()[fin] <= 32 * U).all() and torch.isnan(dx[~fin]).all()
+
+
+def test_activation_gradient_against_differences(device):
+    from speedplusbaseline_amd import _lib as L, ops
+    x = torch.linspace(-6, 6, 512, device="cuda").view(4, 128)
+    d = 1e-5
+    for act in (L.ACT_GELU, L.ACT_GELU_TANH, L.ACT_SILU):
+        P = ops.quant8(x)
+        v = values(P)
+        dx = ops.act8_bwd(torch.ones_like(x), P, act)
+        want = (act_ref(v + d, act) - act_ref(v - d, act)) / (2 * d)      # off by d^2 / 6 and 2^-53 * 6 / d
+        assert ((dx.double() - want).abs() <= 1e-6 + 32 * U).all()
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------------------------------
+def block_step(ops, act, p, x, g, dtype):
+    """y = act(norm(x) W1^T + b1) W2^T + b2 with everything the backward pass needs kept in 8 bits, and all gradients"""
+    n, mean, rstd = ops.layernorm_fwd(x, p["gamma"], p["beta"])
+    w1, w1t = ops.quant8_weight(p["w1"])
+    w2, w2t = ops.quant8_weight(p["w2"])
+    n8 = ops.quant8(n)
+    u = ops.gemm8(n8, w1, bias=p["b1"], dtype=dtype)
+    a, u8 = ops.act8_fwd(u, act)
+    a8 = ops.quant8(a)
+    y = ops.gemm8(a8, w2, bias=p["b2"], dtype=dtype)
+    g8 = ops.quant8(g)
+    dw2 = ops.gemm8_wgrad(g, a8)
+    da = ops.gemm8(g8, w2t, dtype=dtype)
+    du = ops.act8_bwd(da, u8, act)
+    dw1 = ops.gemm8_wgrad(du, n8)
+    dn = ops.gemm8(ops.quant8(du), w1t, dtype=dtype)
+    dx, dgamma, dbeta = ops.layernorm_bwd(dn, x, mean, rstd, p["gamma"])
+    return dict(y=y, dx=dx, dw1=dw1, dw2=dw2, dgamma=dgamma, dbeta=dbeta), dict(n=n, u=u, a=a, da=da, du=du, dn=dn, n8=n8, u8=u8, a8=a8, g8=g8, w1=w1, w2=w2)
+
+
+def block_inputs(M, C, H, dtype):
+    g = torch.Generator().manual_seed(M)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()                      # noqa: E731
+    p = dict(gamma=1 + 0.1 * r(C), beta=0.1 * r(C), w1=r(H, C) / C ** 0.5, b1=0.1 * r(H), w2=r(C, H) / H ** 0.5, b2=0.1 * r(C))
+    return p, r(M, C).to(dtype), (0.01 * r(M, C)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,C,H", [(1, 64, 256), (98, 160, 960), (300, 320, 1001)])
+def test_block_of_all_of_them(device, M, C, H, dtype):
+    """each link against float64 on what the links before it produced, and the whole against the unpacked network: a packed operand is off by at most 2^-4 of an
+    element, at most 3.6 % of a vector's norm (uniform error within a step: 2^-4 / sqrt(3)); five of them meet in dx: 0.2 of its norm"""
+    from speedplusbaseline_amd import _lib as L, ops
+    act = L.ACT_GELU
+    p, x, g = block_inputs(M, C, H, dtype)
+    out, mid = block_step(ops, act, p, x, g, dtype)
+    check_product(mid["n8"], mid["w1"], p["b1"], mid["u"])
+    check_product(mid["a8"], mid["w2"], p["b2"], out["y"])
+    check_wgrad(g, mid["a8"], out["dw2"])
+    check_wgrad(mid["du"], mid["n8"], out["dw1"])
+    w1, w2 = values(mid["w1"]), values(mid["w2"])
+    xd = x.double().requires_grad_()
+    q = {k: v.double().requires_grad_() for k, v in p.items()}
+    n = torch.nn.functional.layer_norm(xd, (C,), q["gamma"], q["beta"], 1e-5)
+    y = act_ref(n @ q["w1"].t() + q["b1"], act) @ q["w2"].t() + q["b2"]
+    y.backward(g.double())
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())            # noqa: E731
+    want = dict(y=y.detach(), dx=xd.grad, dw1=q["w1"].grad, dw2=q["w2"].grad, dgamma=q["gamma"].grad, dbeta=q["beta"].grad)
+    for k in want:
+        assert rel(out[k], want[k]) < 0.2, (k, rel(out[k], want[k]))
+
+
+def test_block_in_a_graph_and_on_another_stream(device):
+    """captured once, replayed with the program's own work between: the same bits as the eager run"""
+    from speedplusbaseline_amd import _lib as L, ops
+    p, x, g = block_inputs(2351, 160, 960, torch.bfloat16)
+    eager, _ = block_step(ops, L.ACT_SILU, p, x, g, torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other, _ = block_step(ops, L.ACT_SILU, p, x, g, torch.bfloat16)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(eager[k], other[k]) for k in eager)
+    xs = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static, _ = block_step(ops, L.ACT_SILU, p, xs, g, torch.bfloat16)
+    for i in range(4):
+        xi = x if i % 2 == 0 else x.flip(0).contiguous()
+        want, _ = block_step(ops, L.ACT_SILU, p, xi, g, torch.bfloat16)
+        xs.copy_(xi)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(static[k], want[k]) for k in want), i
+
+
+def test_two_products_at_once_share_nothing(device):
+    from speedplusbaseline_amd import ops
+    sets = []
+    for i in range(2):
+        A, (B, _) = ops.quant8(data(48, 2304, torch.bfloat16, i)), ops.quant8_weight(data(200, 2304, torch.float32, 10 + i))
+        G = data(5000, 64, torch.bfloat16, 20 + i)
+        X8 = ops.quant8(data(5000, 96, torch.bfloat16, 30 + i))
+        sets.append((A, B, G, X8, ops.gemm8(A, B), ops.gemm8_wgrad(G, X8)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((ops.gemm8(sets[i][0], sets[i][1]), ops.gemm8_wgrad(sets[i][2], sets[i][3])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y, dw in got[i]:
+            assert torch.equal(y, sets[i][4]) and torch.equal(dw, sets[i][5])
