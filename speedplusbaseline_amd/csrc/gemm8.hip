@@ -22,7 +22,9 @@ struct Gemm8Args {
   const unsigned char* A; const unsigned char* As; const unsigned char* B; const unsigned char* Bs;
   const float* bias; void* Y;
   long long M, ldy;
+  long long plane;       // distance of two splits' outputs; 0: one split
   int N, Kp, Sp, bshift, vec;
+  int steps;             // steps of the reduction for each split
 };
 
 template <typename TO> __device__ __forceinline__ void store4(TO* p, const float v[4]);
@@ -31,55 +33,101 @@ template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, const floa
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
-// BM x BN tile, WM x WN waves
-template <int BM, int BN, int WM, int WN, typename TO>
+// 8 of a lane's 32 codes as bfloat16 values.  A and B give the same 8, so any order of the reduction will do.
+__device__ __forceinline__ b16x8_t wide8(const i32x8_t& f, int h, float s) {
+  union { bf2_t p[4]; b16x8_t v; } o;
+  o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h], s, false);
+  o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h], s, true);
+  o.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h + 1], s, false);
+  o.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h + 1], s, true);
+  return o.v;
+}
+__device__ __forceinline__ float scale_of(unsigned byte) { return p8_pow2((int)(byte & 255u) - 127); }
+
+// LDS-DMA (16 / 4 bytes a lane, lane i behind lds_base in order); m0 is not saved: nothing in these kernels uses it
+__device__ __forceinline__ void dma16m(const void* sbase, unsigned voff, unsigned lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4m(const void* sbase, unsigned voff, unsigned lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "memory", "m0");
+}
+
+// bias, rounding and the store of four neighbouring columns of a row
+template <typename TO> __device__ __forceinline__ void put4(const Gemm8Args& g, TO* Y, long long m, int n, const f32x4_t& acc, const float bias[4]) {
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = acc[r] + bias[r];
+  TO* p = Y + m * g.ldy + n;
+  if (g.vec && n + 4 <= g.N) store4<TO>(p, v);
+  else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < g.N) p[r] = from_f<TO>(v[r]);
+  }
+}
+__device__ __forceinline__ void bias4(const Gemm8Args& g, int n, float bias[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) bias[r] = g.bias != nullptr && n + r < g.N ? g.bias[n + r] : 0.f;
+}
+
+constexpr int BAND = 8;      // tile rows that are walked together
+// BM x BN tile, WM x WN waves, a ring of NST stages
+template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) {
-  constexpr bool EXACT = sizeof(TO) == 4;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int STAGE = (BM + BN) * 128, DI = (BM + BN) / 8 / NW;       // DMA instructions of a stage for each wave: 8 rows each
-  constexpr int SI = (BM + BN) / 64;                                    // DMA instructions of four steps' scales: 64 rows each
-  extern __shared__ __attribute__((aligned(16))) char smem[];           // [2] stages, [2] scale tables
+  constexpr int TILE = (BM + BN) * 128, STAGE = TILE + (BM + BN) * 4;   // codes, then the dword of scales that holds this step's
+  constexpr int DI = (BM + BN) / 8 / NW;                                // DMA instructions of a stage for each wave: 8 rows of codes each
+  constexpr int ST = (BM + BN) / 64, SI = (ST + NW - 1) / NW;           // and 64 rows of scales each (a wave too many repeats an instruction)
+  static_assert(DI * 8 * NW == BM + BN && ST * 64 == BM + BN, "whole DMA instructions");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wm = w / WN, wn = w % WN;
-  const int NT = (g.N + BN - 1) / BN;
-  const int lid = xcd_remap(blockIdx.x, gridDim.x);
-  const long long m0 = (long long)(lid / NT) * BM;
-  const int n0 = (lid % NT) * BN;
-  const int KT = g.Kp >> 7;
+  // The 32 workgroups that an XCD runs at a time share one L2: eight tile rows times four tile columns of them fetch 12 tiles a step where a line of
+  // 32 fetches 33 (8192 x 8192 x 8192: 4 TB/s out of the L2s' misses, half the matrix cores' time spent waiting).
+  const int NT = (g.N + BN - 1) / BN, MT = (int)((g.M + BM - 1) / BM);
+  const int tiles = MT * NT, wg = xcd_remap(blockIdx.x, gridDim.x), split = wg / tiles;
+  const int lid = wg - split * tiles, band = lid / (BAND * NT), in = lid - band * (BAND * NT);
+  const int rows = MT - band * BAND < BAND ? MT - band * BAND : BAND;
+  const long long m0 = (long long)(band * BAND + in % rows) * BM;
+  const int n0 = in / rows * BN;
+  const int kbeg = split * g.steps, KT = ((g.Kp >> 7) - kbeg < g.steps ? (g.Kp >> 7) - kbeg : g.steps);     // g.steps is a multiple of 4
 
   // DMA roles: row r of the stage (A rows, then B rows); rows behind the matrix repeat its last one (their results are not stored)
   const unsigned lds0 = lds_addr(smem);
-  const char* abase = reinterpret_cast<const char*>(g.A) + m0 * g.Kp;
-  const char* bbase = reinterpret_cast<const char*>(g.B) + (long long)n0 * g.Kp;
+  const char* abase = reinterpret_cast<const char*>(g.A) + m0 * g.Kp + (long long)kbeg * 128;
+  const char* bbase = reinterpret_cast<const char*>(g.B) + (long long)n0 * g.Kp + (long long)kbeg * 128;
   const int mlast = (int)(g.M - 1 - m0 < BM - 1 ? g.M - 1 - m0 : BM - 1), nlast = g.N - 1 - n0 < BN - 1 ? g.N - 1 - n0 : BN - 1;
   const int slot = ((l & 7) ^ (l >> 3)) << 4;
-  unsigned off[DI];
+  unsigned off[DI], soff[SI];
 #pragma unroll
   for (int i = 0; i < DI; ++i) {
     const int r = (i * NW + w) * 8 + (l >> 3);
     const int rc = r < BM ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
     off[i] = (unsigned)rc * (unsigned)g.Kp + (unsigned)slot;
   }
-  const char* asb = reinterpret_cast<const char*>(g.As) + m0 * g.Sp;
-  const char* bsb = reinterpret_cast<const char*>(g.Bs) + (long long)(n0 >> g.bshift) * g.Sp;
-  auto issue = [&](int kt, int buf) {
-    const unsigned sb = lds0 + (unsigned)(buf * STAGE);
+  const char* asb = reinterpret_cast<const char*>(g.As) + m0 * g.Sp + kbeg;
+  const char* bsb = reinterpret_cast<const char*>(g.Bs) + (long long)(n0 >> g.bshift) * g.Sp + kbeg;
 #pragma unroll
-    for (int i = 0; i < DI; ++i) {
+  for (int i = 0; i < SI; ++i) {
+    const int r = (i * NW + w) % ST * 64 + l;
+    const int rc = r < BM ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
+    soff[i] = (unsigned)(r < BM ? rc : ((n0 + rc) >> g.bshift) - (n0 >> g.bshift)) * (unsigned)g.Sp;
+  }
+  // DMA instruction i of stage kt into buffer `buf`: DI of codes, then SI of scales
+  auto issue1 = [&](int i, int kt, int buf) {
+    const unsigned sb = lds0 + (unsigned)(buf * STAGE);
+    if (i < DI) {
       const int r0 = (i * NW + w) * 8;
-      dma16s((r0 < BM ? abase : bbase) + (size_t)kt * 128, off[i], sb + (unsigned)(r0 * 128));
+      dma16m((r0 < BM ? abase : bbase) + (size_t)kt * 128, off[i < DI ? i : 0], sb + (unsigned)(r0 * 128));
+    } else {
+      const int r0 = ((i - DI) * NW + w) % ST * 64;
+      dma4m((r0 < BM ? asb : bsb) + (kt & ~3), soff[i < DI ? 0 : i - DI], sb + (unsigned)(TILE + r0 * 4));
     }
-    if ((kt & 3) == 0) {
-      for (int i = w; i < SI; i += NW) {
-        const int r = i * 64 + l;
-        const bool isa = i * 64 < BM;
-        const int rc = isa ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
-        // n0 is a multiple of 128 where blocks share scales (BN is): the block of a row is its distance from n0
-        const unsigned so = (unsigned)(isa ? rc : rc >> g.bshift) * (unsigned)g.Sp;
-        dma4s((isa ? asb : bsb) + kt, so, lds0 + (unsigned)(2 * STAGE + ((kt >> 2) & 1) * (BM + BN) * 4 + i * 256));
-      }
-    }
+  };
+  auto issue = [&](int kt, int buf) {
+#pragma unroll
+    for (int i = 0; i < DI + SI; ++i) issue1(i, kt, buf);
   };
 
   f32x4_t acc[TM][TN];
@@ -96,94 +144,177 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
     return f.v;
   };
 
-  issue(0, 0);
-  wait_vmcnt<0>();
-  lds_barrier();
-  unsigned sa[TM], sb[TN];
-  for (int kt = 0; kt < KT; ++kt) {
-    const int buf = kt & 1;
-    if (kt + 1 < KT) issue(kt + 1, buf ^ 1);
-    const char* stage = smem + buf * STAGE;
-    if ((kt & 3) == 0) {
-      const unsigned* tab = reinterpret_cast<const unsigned*>(smem + 2 * STAGE) + ((kt >> 2) & 1) * (BM + BN);
+  // this wave's share of stage kt has landed once only the stages behind it are in flight; behind the barrier everybody's has, and everybody is done
+  // with stage kt - 1, whose buffer takes stage kt + NST - 1
+  auto land = [&](int kt) {
+    if (NST > 2 && kt + NST - 2 < KT) wait_vmcnt<(NST - 2) * (DI + SI)>();
+    else if (NST > 3 && kt + 1 < KT) wait_vmcnt<DI + SI>();
+    else wait_vmcnt<0>();
+    lds_barrier();
+  };
+  const int ao = (wm * TM * 16 + li) * 128, bo = BM * 128 + (wn * TN * 16 + li) * 128;
+  const int ato = TILE + (wm * TM * 16 + li) * 4, bto = TILE + (BM + wn * TN * 16 + li) * 4;
+  for (int s = 0; s < NST - 1 && s < KT; ++s) issue(s, s);
+  int buf = 0;
+  land(0);
+  if constexpr (!EXACT) {
+    // The operands of row tile i + 1 are read while row tile i is multiplied, and the next stage's DMA goes out between them: at the head of the step
+    // its instructions would keep the first operand reads waiting.
+    int sa[TM], sb[TN];
+    constexpr int AHEAD = 1;
+    constexpr int PER = (DI + SI + TM - 1) / TM;
+    for (int kt = 0; kt < KT; ++kt) {
+      if (kt > 0) land(kt);
+      const char* stage = smem + buf * STAGE;
+      const int nbuf = buf == 0 ? NST - 1 : buf - 1;
+      const bool more = kt + NST - 1 < KT;
+      buf = buf == NST - 1 ? 0 : buf + 1;
+      i32x8_t b[TN], a[AHEAD + 1];
+      a[0] = frag(stage + ao);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) sa[i] = tab[(wm * TM + i) * 16 + li];
+      for (int j = 0; j < TN; ++j) b[j] = frag(stage + bo + j * 2048);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) sb[j] = tab[BM + (wn * TN + j) * 16 + li];
-    } else {
+      for (int i = 1; i < AHEAD && i < TM; ++i) a[i] = frag(stage + ao + i * 2048);
+      if ((kt & 3) == 0) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) sa[i] >>= 8;
+        for (int j = 0; j < TN; ++j) sb[j] = *reinterpret_cast<const int*>(stage + bto + j * 64);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) sb[j] >>= 8;
-    }
-    const char* as = stage + (wm * TM * 16 + li) * 128;
-    const char* bs = stage + BM * 128 + (wn * TN * 16 + li) * 128;
-    if constexpr (!EXACT) {
-      i32x8_t b[TN];
+        for (int i = 0; i < TM; ++i) sa[i] = *reinterpret_cast<const int*>(stage + ato + i * 64);
+      } else {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = frag(bs + j * 2048);
+        for (int j = 0; j < TN; ++j) sb[j] = (int)((unsigned)sb[j] >> 8);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] = (int)((unsigned)sa[i] >> 8);
+      }
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const i32x8_t a = frag(as + i * 2048);
+        if (i + AHEAD < TM) a[(i + AHEAD) % (AHEAD + 1)] = frag(stage + ao + (i + AHEAD) * 2048);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a, acc[i][j], 0, 0, 0, (int)sb[j], 0, (int)sa[i]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i % (AHEAD + 1)], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
+        if (more) {
+#pragma unroll
+          for (int q = i * PER; q < (i + 1) * PER && q < DI + SI; ++q) issue1(q, kt + NST - 1, nbuf);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    } else {
-      // 8 of the lane's 32 codes at a time: the same ones of A and B, so any order of the reduction will do
-      auto wide = [&](const i32x8_t& f, int h, float s) {
-        union { bf2_t p[4]; b16x8_t v; } o;
-        o.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h], s, false);
-        o.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h], s, true);
-        o.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h + 1], s, false);
-        o.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * h + 1], s, true);
-        return o.v;
-      };
+    }
+  } else {
+    for (int kt = 0; kt < KT; ++kt) {
+      if (kt > 0) land(kt);
+            if (kt + NST - 1 < KT) issue(kt + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+      const char* stage = smem + buf * STAGE;
+      buf = buf == NST - 1 ? 0 : buf + 1;
       i32x8_t b[TN], a[TM];
       float fa[TM], fb[TN];
+      const int sh = (kt & 3) * 8;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) { b[j] = frag(bs + j * 2048); fb[j] = p8_pow2((int)(sb[j] & 255u) - 127); }
+      for (int j = 0; j < TN; ++j) { b[j] = frag(stage + bo + j * 2048); fb[j] = scale_of(*reinterpret_cast<const unsigned*>(stage + bto + j * 64) >> sh); }
 #pragma unroll
-      for (int i = 0; i < TM; ++i) { a[i] = frag(as + i * 2048); fa[i] = p8_pow2((int)(sa[i] & 255u) - 127); }
+      for (int i = 0; i < TM; ++i) { a[i] = frag(stage + ao + i * 2048); fa[i] = scale_of(*reinterpret_cast<const unsigned*>(stage + ato + i * 64) >> sh); }
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         b16x8_t wb[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) wb[j] = wide(b[j], h, fb[j]);
+        for (int j = 0; j < TN; ++j) wb[j] = wide8(b[j], h, fb[j]);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const b16x8_t wa = wide(a[i], h, fa[i]);
+          const b16x8_t wa = wide8(a[i], h, fa[i]);
 #pragma unroll
           for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], wa, acc[i][j], 0, 0, 0);
         }
       }
     }
-    wait_vmcnt<0>();          // this wave's share of the next stage has landed
-    lds_barrier();            // everybody's has, and everybody is done with this one
   }
 
-  TO* Y = reinterpret_cast<TO*>(g.Y);
+  TO* Y = reinterpret_cast<TO*>(g.Y) + split * g.plane;
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
     const int n = n0 + (wn * TN + j) * 16 + lq * 4;
     float bias[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) bias[r] = g.bias != nullptr && n + r < g.N ? g.bias[n + r] : 0.f;
+    bias4(g, n, bias);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const long long m = m0 + (wm * TM + i) * 16 + li;
-      if (m >= g.M) continue;
-      float v[4];
+      if (m < g.M) put4<TO>(g, Y, m, n, acc[i][j], bias);
+    }
+  }
+}
+
+// Few rows (M <= 16): the product is a stream of B.  A workgroup takes 16 columns of Y and its sixteen waves every sixteenth pair of steps of the reduction:
+// 256 bytes of each row, straight from memory in operand layout, all requested before the first is used.  No wave prefetches; four on each SIMD
+// cover each other.  A comes through L2.  The waves' sums meet in LDS, in order.  (With more rows the half lines that this layout loads of A cost more
+// than the tiles' way through LDS: 48 x 4096 x 9216 took 20 us with three row tiles.)
+constexpr int SKW = 16;
+template <typename TO>
+__global__ __launch_bounds__(SKW * 64) void gemm8_rows_kernel(const Gemm8Args g) {
+  constexpr bool EXACT = sizeof(TO) == 4;
+  __shared__ __attribute__((aligned(16))) f32x4_t part[SKW][64];
+  const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int n0 = blockIdx.x * 16, KT = g.Kp >> 7;
+  const int n = n0 + li < g.N ? n0 + li : g.N - 1;
+  const unsigned char* brow = g.B + (long long)n * g.Kp + lq * 16;
+  const unsigned char* bsc = g.Bs + (long long)(n >> g.bshift) * g.Sp;
+  const long long m = li < g.M ? li : g.M - 1;
+  const unsigned char* arow = g.A + m * g.Kp + lq * 16;
+  const unsigned char* asc = g.As + m * g.Sp;
+  union F { uint4 u[2]; i32x8_t v; };
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int kt = 2 * w; kt < KT; kt += 2 * SKW) {
+    const int k1 = kt + 1 < KT ? kt + 1 : kt;            // an odd number of steps: the last pair is one
+    F b[2], a[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] + bias[r];
-      TO* p = Y + m * g.ldy + n;
-      if (g.vec && n + 4 <= g.N) store4<TO>(p, v);
-      else {
+    for (int u = 0; u < 2; ++u) {
+      const long long o = (long long)(u ? k1 : kt) * 128;
+      b[u].u[0] = *reinterpret_cast<const uint4*>(brow + o);
+      b[u].u[1] = *reinterpret_cast<const uint4*>(brow + o + 64);
+      a[u].u[0] = *reinterpret_cast<const uint4*>(arow + o);
+      a[u].u[1] = *reinterpret_cast<const uint4*>(arow + o + 64);
+    }
+    const unsigned sb = *reinterpret_cast<const unsigned short*>(bsc + kt);            // rows of scales hold a multiple of four
+    const unsigned sa = *reinterpret_cast<const unsigned short*>(asc + kt);
+    __builtin_amdgcn_sched_barrier(0);                                  // left alone, the compiler trades the loads in flight for fewer registers
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < g.N) p[r] = from_f<TO>(v[r]);
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1 && kt + 1 >= KT) break;
+      if constexpr (!EXACT) {
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[u].v, a[u].v, acc, 0, 0, 0, (int)(sb >> (8 * u)), 0, (int)(sa >> (8 * u)));
+      } else {
+        const float fb = scale_of(sb >> (8 * u)), fa = scale_of(sa >> (8 * u));
+#pragma unroll
+        for (int h = 0; h < 4; ++h) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide8(b[u].v, h, fb), wide8(a[u].v, h, fa), acc, 0, 0, 0);
       }
     }
   }
+  part[w][l] = acc;
+  __syncthreads();
+  if (w == 0) {
+    f32x4_t v = part[0][l];
+#pragma unroll
+    for (int k = 1; k < SKW; ++k) v += part[k][l];
+    const int nn = n0 + lq * 4;
+    float bias[4];
+    bias4(g, nn, bias);
+    if (li < g.M) put4<TO>(g, reinterpret_cast<TO*>(g.Y), li, nn, v, bias);
+  }
+}
+
+// Y = the S partial products, in order, + bias: four columns a thread
+template <typename TO> __global__ __launch_bounds__(256) void gemm8_join_kernel(const Gemm8Args g, const float* part, int S) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int q = (g.N + 3) >> 2;
+  const long long m = i / q;
+  const int n = (int)(i - m * q) * 4;
+  if (m >= g.M) return;
+  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < S; ++s) {
+    const float* p = part + s * g.plane + m * (4 * q) + n;        // partial rows hold a multiple of four columns
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v += (f32x4_t){x.x, x.y, x.z, x.w};
+  }
+  float bias[4];
+  bias4(g, n, bias);
+  put4<TO>(g, reinterpret_cast<TO*>(g.Y), m, n, v, bias);
 }
 
 // no reduction (K == 0): the bias alone
@@ -194,13 +325,53 @@ template <typename TO> __global__ __launch_bounds__(256) void gemm8_bias_kernel(
   if (m < g.M) reinterpret_cast<TO*>(g.Y)[m * g.ldy + n] = from_f<TO>(g.bias ? g.bias[n] : 0.f);
 }
 
-template <int BM, int BN, int WM, int WN, typename TO> int run(const Gemm8Args& g, hipStream_t s) {
-  constexpr int LDS = 2 * (BM + BN) * 128 + 2 * (BM + BN) * 4;
-  const long long tiles = (g.M + BM - 1) / BM * ((g.N + BN - 1) / BN);
-  if (tiles > 0x7fffffffll) return SPB_E_SHAPE;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm8_kernel<BM, BN, WM, WN, TO>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int run(const Gemm8Args& g, int S, hipStream_t s) {
+  constexpr int LDS = NST * (BM + BN) * 132;
+  const long long wgs = (g.M + BM - 1) / BM * ((g.N + BN - 1) / BN) * S;
+  if (wgs > 0x7fffffffll) return SPB_E_SHAPE;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm8_kernel<BM, BN, WM, WN, NST, EXACT, TO>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL((gemm8_kernel<BM, BN, WM, WN, TO>), dim3((unsigned)tiles), dim3(WM * WN * 64), LDS, s, g);
+  hipLaunchKernelGGL((gemm8_kernel<BM, BN, WM, WN, NST, EXACT, TO>), dim3((unsigned)wgs), dim3(WM * WN * 64), LDS, s, g);
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+
+constexpr long long ROWS_MAX = 16;
+// How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 282 us, 128 x 128: 301 us) but leave compute units idle below about 192 of
+// them (2352 x 1024 x 1280: 24 against 11 us); 128 x 128 tiles are used down to 128 of those.  Smaller products take 64 x 64 tiles, and where even these are
+// fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up.
+struct Cut { int tile, S, steps; };
+inline Cut cut_of(long long M, int N, int KT) {
+  const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
+  if (t256 >= 192) return {256, 1, (KT + 3) / 4 * 4};
+  if (t128 >= 128) return {128, 1, (KT + 3) / 4 * 4};
+  long long S = t64 >= 256 ? 1 : 256 / t64;
+  const int quads = (KT + 3) / 4;
+  if (S > quads) S = quads;
+  const int per = (int)((quads + S - 1) / S);
+  return {64, (quads + per - 1) / per, per * 4};
+}
+template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hipStream_t s) {
+  if (g.M <= ROWS_MAX) {
+    hipLaunchKernelGGL((gemm8_rows_kernel<TO>), dim3((unsigned)((g.N + 15) / 16)), dim3(SKW * 64), 0, s, g);
+    SPB_CHECK_LAUNCH();
+    return 0;
+  }
+  const Cut c = cut_of(g.M, g.N, g.Kp >> 7);
+  Gemm8Args h = g;
+  h.steps = c.steps;
+  if constexpr (!EXACT) {
+    if (c.tile == 256) return run<256, 256, 2, 4, 2, false, TO>(h, 1, s);
+  }
+  if (c.tile >= 128) return run<128, 128, 2, EXACT ? 2 : 4, EXACT ? 2 : 4, EXACT, TO>(h, 1, s);
+  if (c.S == 1) return run<64, 64, 2, 2, 4, EXACT, TO>(h, 1, s);
+  const long long q = (g.N + 3) / 4, blocks = (g.M * q + 255) / 256;
+  h.Y = ws; h.bias = nullptr; h.ldy = 4 * q; h.plane = g.M * h.ldy; h.vec = 1;
+  const int e = run<64, 64, 2, 2, 4, EXACT, float>(h, c.S, s);
+  if (e) return e;
+  Gemm8Args j = g;
+  j.plane = h.plane;
+  hipLaunchKernelGGL((gemm8_join_kernel<TO>), dim3((unsigned)blocks), dim3(256), 0, s, j, (const float*)ws, c.S);
   SPB_CHECK_LAUNCH();
   return 0;
 }
@@ -209,7 +380,9 @@ template <int BM, int BN, int WM, int WN, typename TO> int run(const Gemm8Args& 
 
 extern "C" long long spb_gemm8_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
-  return 0;
+  if (M <= ROWS_MAX || N == 0 || K == 0) return 0;
+  const Cut c = cut_of(M, N, (K + 127) / 128);
+  return c.S > 1 ? (long long)c.S * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
 extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stream) {
@@ -219,8 +392,8 @@ extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stre
   if (!a->Y) return SPB_E_ARG;
   const int es = dtype == SPB_F32 ? 4 : 2;
   hipStream_t s = (hipStream_t)stream;
-  Gemm8Args g = {a->A, a->As, a->B, a->Bs, a->bias, a->Y, a->M, a->ldy, a->N, p8_cols(a->K), p8_scales(a->K), a->b_block_rows == 128 ? 7 : 0,
-                 ((uintptr_t)a->Y % (4 * es)) == 0 && a->ldy % 4 == 0};
+  Gemm8Args g = {a->A, a->As, a->B, a->Bs, a->bias, a->Y, a->M, a->ldy, 0, a->N, p8_cols(a->K), p8_scales(a->K), a->b_block_rows == 128 ? 7 : 0,
+                 ((uintptr_t)a->Y % (4 * es)) == 0 && a->ldy % 4 == 0, 0};
   if (a->K == 0) {
     const long long blocks = (a->M * a->N + 255) / 256;
     if (blocks > 0x7fffffffll) return SPB_E_SHAPE;
@@ -230,5 +403,7 @@ extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stre
     return 0;
   }
   if (!a->A || !a->As || !a->B || !a->Bs || (((uintptr_t)a->A | (uintptr_t)a->B) & 15) || (((uintptr_t)a->As | (uintptr_t)a->Bs) & 3)) return SPB_E_ARG;
-  return dtype == SPB_F32 ? run<128, 128, 2, 2, float>(g, s) : run<128, 128, 2, 2, bf16_t>(g, s);
+  const long long need = spb_gemm8_bytes(dtype, a->M, a->N, a->K);
+  if (need > 0 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < need)) return SPB_E_ARG;
+  return dtype == SPB_F32 ? product<true, float>(g, a->ws, s) : product<false, bf16_t>(g, a->ws, s);
 }

@@ -60,10 +60,22 @@ template <int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_param(co
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = ln_col<TPR, VEC>(j, i, lane);
-      v[j][i] = p != nullptr ? p[c < C ? c : 0] : other;
+    for (int i = 0; i < 8; ++i) v[j][i] = other;
+  if (p == nullptr) return;
+  const bool whole = VEC && ((uintptr_t)p & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (whole) {
+      const int c = (j * TPR + lane) * 8;
+      ld8<float>(p + (c < C ? c : 0), v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = ln_col<TPR, VEC>(j, i, lane);
+        v[j][i] = p[c < C ? c : 0];
+      }
     }
+  }
 }
 template <typename T, int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_store(T* row, int C, int lane, const float v[NV][8]) {
 #pragma unroll
@@ -307,23 +319,31 @@ __global__ __launch_bounds__(256) void ln_bwd_cols(const spb_layernorm_args_t a,
   out[c] = dg; out[a.C + c] = db;
 }
 
-// dgamma / dbeta (+)= the P partial rows, in order: 64 columns a workgroup, its four waves take a quarter of the rows each
-__global__ __launch_bounds__(256) void ln_join_kernel(const float* part, int P, int C, float* dgamma, float* dbeta, int accumulate) {
-  __shared__ float red[4][64];
+// dgamma / dbeta (+)= the P partial rows, in order: 64 columns a workgroup, its sixteen waves a sixteenth of the rows each, eight requested at a time (a loop
+// of dependent additions waits for memory at every row: 128 rows took 35 us, this form takes 4)
+constexpr int LN_JOIN = 16;
+__global__ __launch_bounds__(LN_JOIN * 64) void ln_join_kernel(const float* part, int P, int C, float* dgamma, float* dbeta, int accumulate) {
+  __shared__ float red[LN_JOIN][64];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const long long n = 2ll * C, c = (long long)blockIdx.x * 64 + l;
+  const long long n = 2ll * C, c = (long long)blockIdx.x * 64 + l, cc = c < n ? c : n - 1;
+  const int per = (P + LN_JOIN - 1) / LN_JOIN, p0 = w * per, p1 = p0 + per < P ? p0 + per : P;
   float v = 0.f;
-  if (c < n) {
-    const int per = (P + 3) >> 2, p1 = (w + 1) * per < P ? (w + 1) * per : P;
-    for (int p = w * per; p < p1; ++p) v += part[p * n + c];
+  for (int p = p0; p < p1; p += 8) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = part[(p + i < p1 ? p + i : p1 - 1) * n + cc];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += p + i < p1 ? x[i] : 0.f;
   }
   red[w][l] = v;
   __syncthreads();
   if (w == 0 && c < n) {
-    v = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < LN_JOIN; ++k) v += red[k][l];
     float* dst = c < C ? dgamma : dbeta;
-    const int cc = (int)(c < C ? c : c - C);
-    if (dst) dst[cc] = (accumulate ? dst[cc] : 0.f) + v;
+    const int o = (int)(c < C ? c : c - C);
+    if (dst) dst[o] = (accumulate ? dst[o] : 0.f) + v;
   }
 }
 
@@ -334,7 +354,8 @@ inline LnShape ln_shape(int C) {
   if (C <= 256) return {16, 2};
   if (C <= 512) return {64, 1};
   if (C <= 1024) return {64, 2};
-  if (C <= 2048) return {64, 4};
+  if (C <= 1536) return {64, 3};
+  if (C <= 2048) return {256, 1};
   if (C <= 4096) return {256, 2};
   return {256, 4};
 }
@@ -351,8 +372,8 @@ template <typename T, bool VEC> void launch_fwd(const spb_layernorm_args_t& a, h
   const dim3 grid((unsigned)(need < LN_FWD_WGS ? need : LN_FWD_WGS)), block(256);
 #define LN_F(TPR, NV) hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, VEC>), grid, block, 0, s, a)
   if (sh.tpr == 16) { if (sh.nv == 1) LN_F(16, 1); else LN_F(16, 2); }
-  else if (sh.tpr == 64) { if (sh.nv == 1) LN_F(64, 1); else if (sh.nv == 2) LN_F(64, 2); else LN_F(64, 4); }
-  else { if (sh.nv == 2) LN_F(256, 2); else LN_F(256, 4); }
+  else if (sh.tpr == 64) { if (sh.nv == 1) LN_F(64, 1); else if (sh.nv == 2) LN_F(64, 2); else LN_F(64, 3); }
+  else { if (sh.nv == 1) LN_F(256, 1); else if (sh.nv == 2) LN_F(256, 2); else LN_F(256, 4); }
 #undef LN_F
 }
 template <typename T, bool VEC, bool SUMS> void launch_bwd(const spb_layernorm_args_t& a, hipStream_t s) {
@@ -360,8 +381,8 @@ template <typename T, bool VEC, bool SUMS> void launch_bwd(const spb_layernorm_a
   const dim3 grid((unsigned)ln_bwd_parts(a.M, a.C)), block(256);
 #define LN_B(TPR, NV) hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV, VEC, SUMS>), grid, block, 0, s, a)
   if (sh.tpr == 16) { if (sh.nv == 1) LN_B(16, 1); else LN_B(16, 2); }
-  else if (sh.tpr == 64) { if (sh.nv == 1) LN_B(64, 1); else if (sh.nv == 2) LN_B(64, 2); else LN_B(64, 4); }
-  else { if (sh.nv == 2) LN_B(256, 2); else LN_B(256, 4); }
+  else if (sh.tpr == 64) { if (sh.nv == 1) LN_B(64, 1); else if (sh.nv == 2) LN_B(64, 2); else LN_B(64, 3); }
+  else { if (sh.nv == 1) LN_B(256, 1); else if (sh.nv == 2) LN_B(256, 2); else LN_B(256, 4); }
 #undef LN_B
 }
 
@@ -433,7 +454,7 @@ extern "C" int spb_layernorm_bwd(int dtype, const spb_layernorm_args_t* a, spb_s
   }
   SPB_CHECK_LAUNCH();
   if (sums) {
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((2ll * a->C + 63) / 64)), dim3(256), 0, s, a->part, P, a->C, a->dgamma, a->dbeta, a->accumulate);
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((2ll * a->C + 63) / 64)), dim3(LN_JOIN * 64), 0, s, a->part, P, a->C, a->dgamma, a->dbeta, a->accumulate);
     SPB_CHECK_LAUNCH();
   }
   return 0;

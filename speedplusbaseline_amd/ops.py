@@ -2,6 +2,7 @@
 want a single fused op).  Tensors are device memory only; all arithmetic happens in libspb_hip.so.
 """
 import ctypes as C
+import os
 
 import torch
 
@@ -323,211 +324,227 @@ def fc_wgrad_update(gT, xT, M, kind, params, grads=None, m=None, v=None, gmul=No
 # ---- layer norm, 8-bit linear layers and checkpoints ---------------------------------------------------------------------------------
 # Operands are 2-D with contiguous columns and any row stride.  Like every function of this file they enqueue on the current stream and build no
 # autograd graph: the backward pass is the explicit *_bwd / *_wgrad call.  They run on the device of their tensors, whichever is current.
+# A call on a few rows is bound by this file, not by its kernel (12-22 us with the helpers above, 7-12 us like this): devices are compared as
+# indices, argument structs are filled by position, and addresses are plain integers.
+
+_TUNED = bool(os.environ.get("SPB_DEBUG") or os.environ.get("SPB_TUNING_LIB"))
+
+
+def _lib8(dtype):
+    if dtype is torch.float16:
+        return L._lib_f16 or L.lib_f16()
+    return L._lib if L._lib is not None and not _TUNED and L._tuning_depth == 0 else L.lib()
+
 
 def _call(dev, fn, what, *args):
-    if dev.index == torch.cuda.current_device():
-        L.check(fn(*args, _stream()), what)
+    if dev == torch.cuda.current_device():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))     # current_stream(dev).cuda_stream without the 3 us of its object
+        if code:
+            L.check(code, what)
     else:
         with torch.cuda.device(dev):
-            L.check(fn(*args, _stream()), what)
+            L.check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
 
 
-def _mat(t, name, dev=None, out=False):
-    """2-D operand: device memory, contiguous columns, one of the three types; returns its row stride"""
-    if not t.is_cuda:
-        raise RuntimeError("speedplusbaseline_amd ops run on the GPU only (got a %s tensor for %s)" % (t.device, name))
-    if dev is not None and t.device != dev:
-        raise RuntimeError("%s is on %s, the other operands on %s" % (name, t.device, dev))
-    if t.dtype not in _DT:
+def _mat(t, name, dev=None):
+    """2-D operand: device memory, contiguous columns, one of the three types.  Returns (device, rows, columns, row stride, type code)."""
+    code, d = _DT.get(t.dtype), t.get_device()
+    if code is None:
         raise RuntimeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise RuntimeError("%s must be 2-D with contiguous columns, got shape %s, strides %s" % (name, tuple(t.shape), t.stride()))
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if out and ld < t.shape[1]:
+    if d < 0:
+        raise RuntimeError("speedplusbaseline_amd ops run on the GPU only (got a %s tensor for %s)" % (t.device, name))
+    if dev is not None and d != dev:
+        raise RuntimeError("%s is on device %d, the other operands on %d" % (name, d, dev))
+    if t.dim() != 2:
+        raise RuntimeError("%s must be 2-D, got shape %s" % (name, tuple(t.shape)))
+    (rows, cols), (ld, one) = t.shape, t.stride()
+    if one != 1 and cols > 1:
+        raise RuntimeError("the columns of %s must be contiguous, got strides %s" % (name, t.stride()))
+    return d, rows, cols, ld if rows > 1 else cols, code
+
+
+def _like(t, shape, dtype, name, dev):
+    """an operand or output of a known shape and type; returns its row stride"""
+    if t.get_device() != dev or t.dtype != dtype or tuple(t.shape) != shape:
+        raise RuntimeError("%s must be %s %s on device %s, got %s %s on %s" % (name, dtype, shape, dev, t.dtype, tuple(t.shape), t.device))
+    return _mat(t, name)[3]
+
+
+def _out(t, shape, dtype, name, dev):
+    ld = _like(t, shape, dtype, name, dev)
+    if ld < shape[1]:
         raise RuntimeError("the rows of %s overlap" % name)
     return ld
 
 
-def _like(t, shape, dtype, name, dev):
-    if t.device != dev or t.dtype != dtype or tuple(t.shape) != tuple(shape):
-        raise RuntimeError("%s must be %s %s on %s, got %s %s on %s" % (name, dtype, tuple(shape), dev, t.dtype, tuple(t.shape), t.device))
-
-
 def _vec(t, n, name, dev):
-    """contiguous float32 vector of n elements, or None"""
+    """address of a contiguous float32 vector of n elements, or None"""
     if t is None:
-        return
-    _like(t, (n,), torch.float32, name, dev)
-    if not t.is_contiguous():
-        raise RuntimeError("%s must be contiguous" % name)
+        return None
+    if t.get_device() != dev or t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError("%s must be a contiguous float32 [%d] on device %s, got %s %s on %s" % (name, n, dev, t.dtype, tuple(t.shape), t.device))
+    return t.data_ptr()
 
 
 def layernorm_fwd(X, gamma=None, beta=None, eps=1e-5, Y=None):
     """Layer norm over the columns of X [M, C]: returns (Y, mean, rstd); mean and rstd (float32 [M]) are what layernorm_bwd needs.  gamma / beta:
     float32 [C] or None (1 / 0).  Y: optional output of X's type, may be X itself."""
-    ldx = _mat(X, "X")
-    dev, (M, Cn) = X.device, X.shape
+    dev, M, Cn, ldx, code = _mat(X, "X")
     if Cn < 1:
         raise RuntimeError("layernorm needs at least one column")
-    _vec(gamma, Cn, "gamma", dev); _vec(beta, Cn, "beta", dev)
     if Y is None:
-        Y = torch.empty(M, Cn, dtype=X.dtype, device=dev)
+        Y, ldy = X.new_empty((M, Cn)), Cn
     else:
-        _like(Y, X.shape, X.dtype, "Y", dev)
-    stats = torch.empty(2, M, dtype=torch.float32, device=dev)
-    mean, rstd = stats[0], stats[1]
-    a = A8.LayerNormArgs()
-    a.X, a.Y, a.gamma, a.beta, a.mean, a.rstd = _ptr(X), _ptr(Y), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd)
-    a.M, a.C, a.ldx, a.ldy, a.eps = M, Cn, ldx, _mat(Y, "Y", dev, out=True), eps
-    _call(dev, lib_of(X).spb_layernorm_fwd, "spb_layernorm_fwd", dtype_code(X, True), C.byref(a))
+        ldy = _out(Y, (M, Cn), X.dtype, "Y", dev)
+    mean, rstd = torch.empty((2, M), dtype=torch.float32, device=X.device).unbind(0)
+    a = A8.LayerNormArgs(X.data_ptr(), None, _vec(gamma, Cn, "gamma", dev), _vec(beta, Cn, "beta", dev), Y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+                         None, None, None, 0, M, ldx, 0, ldy, Cn, eps, 0)
+    _call(dev, _lib8(X.dtype).spb_layernorm_fwd, "spb_layernorm_fwd", code, C.byref(a))
     return Y, mean, rstd
 
 
 def layernorm_bwd(G, X, mean, rstd, gamma=None, dgamma=None, dbeta=None, dX=None, param_grads=True):
     """Backward of layernorm_fwd: returns (dX, dgamma, dbeta).  dgamma / dbeta given: accumulated into (both or neither), otherwise new;
     param_grads=False: not computed (None).  dX: optional output, may be G itself."""
-    ldg, ldx = _mat(G, "G"), _mat(X, "X", G.device)
-    dev, (M, Cn) = X.device, X.shape
+    dev, M, Cn, ldx, code = _mat(X, "X")
+    ldg = _like(G, (M, Cn), X.dtype, "G", dev)
     if Cn < 1:
         raise RuntimeError("layernorm needs at least one column")
-    _like(G, X.shape, X.dtype, "G", dev)
-    _vec(gamma, Cn, "gamma", dev); _vec(mean, M, "mean", dev); _vec(rstd, M, "rstd", dev)
-    _vec(dgamma, Cn, "dgamma", dev); _vec(dbeta, Cn, "dbeta", dev)
     if (dgamma is None) != (dbeta is None) or (dgamma is not None and not param_grads):
         raise RuntimeError("dgamma and dbeta are accumulated into together")
+    if mean is None or rstd is None:
+        raise RuntimeError("layernorm_bwd needs the forward's mean and rstd")
     if dX is None:
-        dX = torch.empty(M, Cn, dtype=X.dtype, device=dev)
+        dX, ldd = X.new_empty((M, Cn)), Cn
     else:
-        _like(dX, X.shape, X.dtype, "dX", dev)
-    lib = lib_of(X)
-    a = A8.LayerNormArgs()
-    a.X, a.G, a.Y, a.gamma, a.mean, a.rstd = _ptr(X), _ptr(G), _ptr(dX), _ptr(gamma), _ptr(mean), _ptr(rstd)
-    a.M, a.C, a.ldx, a.ldg, a.ldy = M, Cn, ldx, ldg, _mat(dX, "dX", dev, out=True)
+        ldd = _out(dX, (M, Cn), X.dtype, "dX", dev)
+    lib = _lib8(X.dtype)
+    cap, part, accumulate = 0, None, 0
     if param_grads:
-        a.accumulate = 0 if dgamma is None else 1
+        accumulate = 0 if dgamma is None else 1
         if dgamma is None:
-            dgamma, dbeta = torch.empty(Cn, dtype=torch.float32, device=dev), torch.empty(Cn, dtype=torch.float32, device=dev)
-        a.part_cap = lib.spb_layernorm_bwd_floats(M, Cn)
-        part = torch.empty(a.part_cap, dtype=torch.float32, device=dev)
-        a.part, a.dgamma, a.dbeta = _ptr(part), _ptr(dgamma), _ptr(dbeta)
-    _call(dev, lib.spb_layernorm_bwd, "spb_layernorm_bwd", dtype_code(X, True), C.byref(a))
+            dgamma, dbeta = torch.empty((2, Cn), dtype=torch.float32, device=X.device).unbind(0)
+        cap = lib.spb_layernorm_bwd_floats(M, Cn)
+        part = torch.empty(cap, dtype=torch.float32, device=X.device)
+    a = A8.LayerNormArgs(X.data_ptr(), G.data_ptr(), _vec(gamma, Cn, "gamma", dev), None, dX.data_ptr(), _vec(mean, M, "mean", dev),
+                         _vec(rstd, M, "rstd", dev), _vec(dgamma, Cn, "dgamma", dev), _vec(dbeta, Cn, "dbeta", dev),
+                         None if part is None else part.data_ptr(), cap, M, ldx, ldg, ldd, Cn, 0.0, accumulate)
+    _call(dev, lib.spb_layernorm_bwd, "spb_layernorm_bwd", code, C.byref(a))
     return dX, dgamma, dbeta
 
 
 class Packed8:
     """A matrix in e4m3 codes with one power-of-two scale for each block of 128 (include/spb_hip.h "8-bit packing"): codes uint8 [rows, K rounded up to
     128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight)."""
-    __slots__ = ("codes", "scales", "K", "block_rows")
+    __slots__ = ("_codes", "_scales", "_K", "_block_rows", "_rows", "_dev")
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    K = property(lambda self: self._K)
+    block_rows = property(lambda self: self._block_rows)
+    shape = property(lambda self: (self._rows, self._K))
 
     def __init__(self, codes, scales, K, block_rows):
-        self.codes, self.scales, self.K, self.block_rows = codes, scales, K, block_rows
+        kb = (K + 127) // 128
+        if block_rows not in (1, 128) or K < 0 or codes.dim() != 2:
+            raise RuntimeError("Packed8: block_rows must be 1 or 128 and the codes a matrix")
+        rows = codes.shape[0]
+        for t, shape in ((codes, (rows, kb * 128)), (scales, ((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
+                raise RuntimeError("Packed8: codes and scales do not fit a packed [%d, %d] matrix" % (rows, K))
+        self._set(codes, scales, K, block_rows, rows)
+
+    def _set(self, codes, scales, K, block_rows, rows):
+        self._codes, self._scales, self._K, self._block_rows, self._rows, self._dev = codes, scales, K, block_rows, rows, codes.get_device()
+        return self
 
     @staticmethod
     def empty(rows, K, block_rows, device):
         kb = (K + 127) // 128
-        return Packed8(torch.empty(rows, kb * 128, dtype=torch.uint8, device=device),
-                       torch.empty((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4, dtype=torch.uint8, device=device), K, block_rows)
-
-    @property
-    def shape(self):
-        return (self.codes.shape[0], self.K)
+        return Packed8.__new__(Packed8)._set(torch.empty((rows, kb * 128), dtype=torch.uint8, device=device),
+                                             torch.empty(((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4), dtype=torch.uint8, device=device),
+                                             K, block_rows, rows)
 
 
-def _packed(P, name, dev, block_rows=None):
+def _packed(P, name, dev=None, block_rows=None):
+    """checks a Packed8 operand; returns its device"""
     if not isinstance(P, Packed8):
         raise RuntimeError("%s must be a Packed8 (quant8 / quant8_weight), got %s" % (name, type(P).__name__))
-    if block_rows is not None and P.block_rows != block_rows:
+    if block_rows is not None and P._block_rows != block_rows:
         raise RuntimeError("%s must be packed in blocks of %d x 128" % (name, block_rows))
-    rows, kb = P.codes.shape[0], (P.K + 127) // 128
-    for t, shape in ((P.codes, (rows, kb * 128)), (P.scales, ((rows + P.block_rows - 1) // P.block_rows, (kb + 3) // 4 * 4))):
-        if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous():
-            raise RuntimeError("%s: codes and scales do not fit a packed [%d, %d] matrix" % (name, rows, P.K))
-        if not t.is_cuda or (dev is not None and t.device != dev):
-            raise RuntimeError("%s is on %s, expected %s" % (name, t.device, dev or "a GPU"))
+    if P._dev < 0 or (dev is not None and P._dev != dev):
+        raise RuntimeError("%s is on %s, expected %s" % (name, P._codes.device, "a GPU" if dev is None else "device %d" % dev))
+    return P._dev
 
 
 def quant8(X):
     """X [M, K] packed in blocks of 1 x 128: operand of gemm8 and checkpoint for gemm8_wgrad"""
-    ldx = _mat(X, "X")
-    M, K = X.shape
+    dev, M, K, ldx, code = _mat(X, "X")
     P = Packed8.empty(M, K, 1, X.device)
-    _call(X.device, lib_of(X).spb_pack8_rows, "spb_pack8_rows", dtype_code(X, True), _ptr(X), ldx, M, K, _ptr(P.codes), _ptr(P.scales))
+    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, P._codes.data_ptr(), P._scales.data_ptr())
     return P
 
 
 def quant8_weight(W, transpose=True):
     """W [N, K] packed in blocks of 128 x 128: (operand of Y = X W^T, packed transpose for dX = G W or None)"""
-    ldw = _mat(W, "W")
-    N, K = W.shape
+    dev, N, K, ldw, code = _mat(W, "W")
     P = Packed8.empty(N, K, 128, W.device)
     T = Packed8.empty(K, N, 128, W.device) if transpose else None
-    _call(W.device, lib_of(W).spb_pack8_weight, "spb_pack8_weight", dtype_code(W, True), _ptr(W), ldw, N, K, _ptr(P.codes), _ptr(P.scales),
-          _ptr(T.codes) if transpose else None, _ptr(T.scales) if transpose else None)
+    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, P._codes.data_ptr(), P._scales.data_ptr(),
+          T._codes.data_ptr() if transpose else None, T._scales.data_ptr() if transpose else None)
     return P, T
 
 
 def dequant8(P, dtype=torch.bfloat16, Y=None):
     """the values of a Packed8 (exact in bfloat16 and float32)"""
-    _packed(P, "P", None)
-    dev = P.codes.device
+    dev = _packed(P, "P")
     if Y is None:
-        Y = torch.empty(P.shape, dtype=dtype, device=dev)
-    else:
-        _like(Y, P.shape, dtype, "Y", dev)
-    ldy = _mat(Y, "Y", dev, out=True)
-    _call(dev, lib_of(Y).spb_unpack8, "spb_unpack8", dtype_code(Y, True), _ptr(P.codes), _ptr(P.scales), P.block_rows, P.shape[0], P.K, _ptr(Y), ldy)
+        Y = torch.empty(P.shape, dtype=dtype, device=P._codes.device)
+    ldy = _out(Y, P.shape, dtype, "Y", dev)
+    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], P._codes.data_ptr(), P._scales.data_ptr(), P._block_rows, P._rows, P._K, Y.data_ptr(), ldy)
     return Y
 
 
 def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
     """Y [M, N] = A [M, K] (quant8) times the transpose of B [N, K] (quant8_weight or quant8) + bias (float32 [N]).  dtype float32: the products run
     through the bfloat16 matrix instructions, where they are exact; 16-bit types: through the 8-bit ones."""
-    _packed(A, "A", None, 1)
-    dev = A.codes.device
+    dev = _packed(A, "A", None, 1)
     _packed(B, "B", dev)
-    if A.K != B.K:
-        raise RuntimeError("gemm8: A has %d columns, B has %d" % (A.K, B.K))
-    M, N = A.shape[0], B.shape[0]
-    _vec(bias, N, "bias", dev)
+    if A._K != B._K:
+        raise RuntimeError("gemm8: A has %d columns, B has %d" % (A._K, B._K))
+    M, N, K = A._rows, B._rows, A._K
+    if dtype not in _DT:
+        raise RuntimeError("gemm8 writes float32, bfloat16 or float16, not %s" % dtype)
     if Y is None:
-        Y = torch.empty(M, N, dtype=dtype, device=dev)
+        Y, ldy = torch.empty((M, N), dtype=dtype, device=A._codes.device), N
     else:
-        _like(Y, (M, N), dtype, "Y", dev)
-    a = A8.Gemm8Args()
-    a.ldy = _mat(Y, "Y", dev, out=True)
-    a.A, a.As, a.B, a.Bs, a.bias, a.Y = _ptr(A.codes), _ptr(A.scales), _ptr(B.codes), _ptr(B.scales), _ptr(bias), _ptr(Y)
-    a.M, a.N, a.K, a.b_block_rows = M, N, A.K, B.block_rows
-    lib, code = lib_of(Y), dtype_code(Y, True)
-    a.ws_bytes = lib.spb_gemm8_bytes(code, M, N, A.K)
-    if a.ws_bytes > 0:
-        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
-        a.ws = _ptr(ws)
+        ldy = _out(Y, (M, N), dtype, "Y", dev)
+    lib, code = _lib8(dtype), _DT[dtype]
+    need = lib.spb_gemm8_bytes(code, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=A._codes.device) if need > 0 else None
+    a = A8.Gemm8Args(A._codes.data_ptr(), A._scales.data_ptr(), B._codes.data_ptr(), B._scales.data_ptr(), _vec(bias, N, "bias", dev), Y.data_ptr(),
+                     None if ws is None else ws.data_ptr(), need, M, ldy, N, K, B._block_rows)
     _call(dev, lib.spb_gemm8, "spb_gemm8", code, C.byref(a))
     return Y
 
 
 def gemm8_wgrad(G, X8, dW=None):
     """dW [N, K] (float32) = transpose of G [M, N] times the checkpoint X8 (quant8 of the layer's input [M, K]); dW given: accumulated into"""
-    ldg = _mat(G, "G")
-    dev = G.device
+    dev, M, N, ldg, code = _mat(G, "G")
     _packed(X8, "X8", dev, 1)
-    (M, N), K = G.shape, X8.K
-    if X8.shape[0] != M:
-        raise RuntimeError("gemm8_wgrad: G has %d rows, X8 has %d" % (M, X8.shape[0]))
-    a = A8.Wgrad8Args()
-    a.accumulate = 0 if dW is None else 1
+    K = X8._K
+    if X8._rows != M:
+        raise RuntimeError("gemm8_wgrad: G has %d rows, X8 has %d" % (M, X8._rows))
+    accumulate = 0 if dW is None else 1
     if dW is None:
-        dW = torch.empty(N, K, dtype=torch.float32, device=dev)
+        dW, ldw = torch.empty((N, K), dtype=torch.float32, device=G.device), K
     else:
-        _like(dW, (N, K), torch.float32, "dW", dev)
-    a.ldw = _mat(dW, "dW", dev, out=True)
-    a.G, a.X, a.Xs, a.dW = _ptr(G), _ptr(X8.codes), _ptr(X8.scales), _ptr(dW)
-    a.M, a.N, a.K, a.ldg = M, N, K, ldg
-    lib, code = lib_of(G), dtype_code(G, True)
-    a.ws_bytes = lib.spb_gemm8_wgrad_bytes(code, M, N, K)
-    if a.ws_bytes > 0:
-        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
-        a.ws = _ptr(ws)
+        ldw = _out(dW, (N, K), torch.float32, "dW", dev)
+    lib = _lib8(G.dtype)
+    need = lib.spb_gemm8_wgrad_bytes(code, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=G.device) if need > 0 else None
+    a = A8.Wgrad8Args(G.data_ptr(), X8._codes.data_ptr(), X8._scales.data_ptr(), dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
+                      N, K, accumulate)
     _call(dev, lib.spb_gemm8_wgrad, "spb_gemm8_wgrad", code, C.byref(a))
     return dW
 
@@ -540,32 +557,28 @@ def _act8(act):
 def act8_fwd(X, act, Y=None):
     """(Y, P): Y = act(X) and P = X in 8 bits, the checkpoint act8_bwd reads.  Y: optional output of X's type, may be X itself."""
     _act8(act)
-    ldx = _mat(X, "X")
-    dev, (M, K) = X.device, X.shape
+    dev, M, K, ldx, code = _mat(X, "X")
     if Y is None:
-        Y = torch.empty(M, K, dtype=X.dtype, device=dev)
+        Y, ldy = X.new_empty((M, K)), K
     else:
-        _like(Y, X.shape, X.dtype, "Y", dev)
-    P = Packed8.empty(M, K, 1, dev)
-    _call(dev, lib_of(X).spb_act8_fwd, "spb_act8_fwd", dtype_code(X, True), act, _ptr(X), ldx, _ptr(Y), _mat(Y, "Y", dev, out=True), M, K,
-          _ptr(P.codes), _ptr(P.scales))
+        ldy = _out(Y, (M, K), X.dtype, "Y", dev)
+    P = Packed8.empty(M, K, 1, X.device)
+    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, P._codes.data_ptr(), P._scales.data_ptr())
     return Y, P
 
 
 def act8_bwd(G, P, act, dX=None):
     """dX = G * act'(value of the checkpoint P).  dX: optional output of G's type, may be G itself."""
     _act8(act)
-    ldg = _mat(G, "G")
-    dev, (M, K) = G.device, G.shape
+    dev, M, K, ldg, code = _mat(G, "G")
     _packed(P, "P", dev, 1)
-    if P.shape != (M, K):
+    if P._rows != M or P._K != K:
         raise RuntimeError("act8_bwd: G is %s, the checkpoint %s" % ((M, K), P.shape))
     if dX is None:
-        dX = torch.empty(M, K, dtype=G.dtype, device=dev)
+        dX, ldd = G.new_empty((M, K)), K
     else:
-        _like(dX, G.shape, G.dtype, "dX", dev)
-    _call(dev, lib_of(G).spb_act8_bwd, "spb_act8_bwd", dtype_code(G, True), act, _ptr(G), ldg, _ptr(P.codes), _ptr(P.scales), _ptr(dX),
-          _mat(dX, "dX", dev, out=True), M, K)
+        ldd = _out(dX, (M, K), G.dtype, "dX", dev)
+    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, P._codes.data_ptr(), P._scales.data_ptr(), dX.data_ptr(), ldd, M, K)
     return dX
 
 
