@@ -5,21 +5,24 @@
 // the scale belongs to (m, 128 columns): along the reduction it changes with every step, which is why the 8-bit instructions, whose scale covers 32
 // steps of the reduction, do not fit.  G keeps all its bits: it is split by truncation into 1 (bfloat16), 2 (half: 8 + 3 bits) or 3 (float32: 8 + 8 + 8 bits)
 // bfloat16 pieces with an exact sum.
-//   * 128 x 128 tiles of dW, four waves of 64 x 64; stages of 64 rows in LDS, read with the transpose load ds_read_b64_tr_b16.
+//   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, or 128 x 128 with four of 64 x 64.  Stages of R rows (64; 32 with more than one piece) in LDS, two of
+//     them, read with the transpose load ds_read_b64_tr_b16.
+//   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
 //   * Few tiles and many rows: the rows are split over workgroups, each stores its partial tile, and a second launch adds them in order.
+// LDS rows hold TW columns without padding (the DMA image is linear).  The transpose load reads 32 bytes of 16 rows, r = 8 q + 0 .. 3 (+ 4): the 32-byte
+// pairs of a row are XOR-swizzled with (r & 3) + 4 ((r >> 3) & 1), which spreads them over all banks.
 #include "pack8.h"
 
 namespace {
 
 typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
-constexpr int WT = 128, WR = 64, WLD = WT + 8;       // tile, rows of a stage, row stride in LDS (elements)
 
 struct Wgrad8Args {
   const void* G; const unsigned char* X; const unsigned char* Xs; float* out;
   long long M, ldg, ldo, plane;                        // plane: distance of two splits' outputs (0: a single one)
-  long long rows;                                      // rows of a split, a multiple of WR
-  int N, K, Kp, Sp, NT, KT, accumulate;
+  long long rows;                                      // rows of a split, a multiple of 64
+  int N, K, Kp, Sp, NT, KT, accumulate, vec;           // vec: 16-byte stores fit the output
 };
 
 // bfloat16 pieces of 8 gradients: piece p of element i in out[p]
@@ -41,126 +44,224 @@ template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 
     out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
   }
 }
+__device__ __forceinline__ int wg_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-template <typename T, int P, bool VEC>
-__global__ __launch_bounds__(256) void wgrad8_kernel(const Wgrad8Args g) {
-  __shared__ __attribute__((aligned(16))) bf16_t Gs[P][WR * WLD];
-  __shared__ __attribute__((aligned(16))) bf16_t Xl[WR * WLD];
-  const int t = threadIdx.x, l = t & 63, w = t >> 6, li = l & 15, lq = l >> 4;
-  const int wn = w >> 1, wk = w & 1;
+// WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  DMA: G straight to LDS (P == 1, aligned rows); VEC: aligned rows through registers
+template <typename T, int P, bool DMA, bool VEC, int WN, int WK, int TN, int TK>
+__global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g) {
+  constexpr int TW = WN * TN * 16, NW = WN * WK, NTH = NW * 64;
+  static_assert(WK * TK * 16 == TW && (!DMA || P == 1), "square tiles; DMA does not split");
+  constexpr int R = P == 1 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB, STAGE = (P + 1) * PLANE;
+  constexpr int DI = PLANE / 1024 / NW, RPI = 1024 / ROWB;              // DMA instructions of a stage for each wave, rows each covers
+  constexpr int XL = TW / 16, XR = NTH / XL, XP = R / XR;               // lanes of a row of codes (16 each), rows of a pass, passes
+  constexpr int GL = TW / 8, GRW = NTH / GL, GP = R / GRW;              // the same for 8 gradients a lane
+  extern __shared__ __attribute__((aligned(16))) char smem[];           // two stages: P planes of G, one of X
+  const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wn = w / WK, wk = w % WK;
   const int lid = xcd_remap(blockIdx.x, gridDim.x);     // the tiles of a split read the same rows: one XCD, back to back
   const int tiles = g.NT * g.KT, tile = lid % tiles, split = lid / tiles;
-  const int n0 = (tile / g.KT) * WT, k0 = (tile % g.KT) * WT;
+  const int n0 = (tile / g.KT) * TW, k0 = (tile % g.KT) * TW;
   const long long mb = (long long)split * g.rows, me = mb + g.rows < g.M ? mb + g.rows : g.M;
-  const int cv = t & 15, r0 = t >> 4;                    // this thread's 8 columns and its first row of a stage
-  const int kb = k0 >> 7;
+  const int nst = (int)((me - mb + R - 1) / R);
 
-  f32x4_t acc[4][4];
+  // ---- staging
+  const unsigned lds0 = lds_addr(smem);
+  const int drow = w * RPI + l / (64 / RPI), dslot = l % (64 / RPI);                         // DMA: this lane's row of the first instruction, its 16-byte slot
+  int dcol = n0 + (((dslot >> 1) ^ wg_swz(drow)) * 2 + (dslot & 1)) * 8;                       // NW * RPI is a multiple of 16: the swizzle is the same in all
+  dcol = dcol < g.N ? dcol : g.N - 8;                                                        // columns behind the matrix: any (not stored)
+  const int xr = t / XL, xc = (t % XL) * 16;
+  const int xk = k0 + xc < g.Kp ? k0 + xc : g.Kp - 16;
+  const int gr = t / GL, gc = (t % GL) * 8;
+  uint4 xq[XP];
+  unsigned char xs[XP];
+  Raw8<T> graw[DMA ? 1 : GP];
+  auto fetch = [&](int st, int buf) {                    // requests stage st (its G by DMA into buffer `buf`)
+    const long long m = mb + (long long)st * R;
+    const int last = (int)(me - 1 - m < R - 1 ? me - 1 - m : R - 1);
+    if constexpr (DMA) {
+      const char* base = reinterpret_cast<const char*>(g.G) + m * g.ldg * 2;
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+      for (int i = 0; i < DI; ++i) {
+        const int r = drow + i * (NW * RPI), rc = r < last ? r : last;
+        dma16s(base, ((unsigned)rc * (unsigned)g.ldg + (unsigned)dcol) * 2u, lds0 + (unsigned)(buf * STAGE + (i * NW + w) * 1024));
+      }
+    } else {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < GP; ++i) {
+        const int r = gr + i * GRW, rc = r < last ? r : last;
+        const T* row = reinterpret_cast<const T*>(g.G) + (m + rc) * g.ldg;
+        const int n = n0 + gc;
+        if (VEC) {
+          graw[i] = ldraw<T>(row + (n < g.N ? n : 0));
+        } else {
+          T e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = row[n + j < g.N ? n + j : 0];
+          __builtin_memcpy(&graw[i], e, sizeof(graw[i]));
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < XP; ++i) {
+      const int r = xr + i * XR, rc = r < last ? r : last;
+      xq[i] = *reinterpret_cast<const uint4*>(g.X + (m + rc) * g.Kp + xk);
+      xs[i] = g.Xs[(m + rc) * g.Sp + (xk >> 7)];
+    }
+  };
+  auto commit = [&](int st, int buf) {                   // what came through registers goes to LDS; rows behind the last one as zeros
+    const long long left = me - (mb + (long long)st * R);
+    char* sb = smem + buf * STAGE;
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int i = 0; i < GP; ++i) {
+        const int r = gr + i * GRW;
+        float v[8];
+        cvt8(graw[i], v);
+        uint4 piece[P];
+        split8<P>(v, piece);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          *reinterpret_cast<uint4*>(sb + p * PLANE + r * ROWB + (((gc >> 4) ^ wg_swz(r)) << 5) + ((gc & 8) << 1)) = r < left ? piece[p] : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < XP; ++i) {
+      const int r = xr + i * XR;
+      const float s = p8_pow2((int)xs[i] - 127);
+      const unsigned q[4] = {xq[i].x, xq[i].y, xq[i].z, xq[i].w};
+      union { bf2_t h[8]; uint4 u[2]; } x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? q[j] : 0u, s, false);
+        x.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? q[j] : 0u, s, true);
+      }
+      char* p = sb + P * PLANE + r * ROWB + (((xc >> 4) ^ wg_swz(r)) << 5);
+      *reinterpret_cast<uint4*>(p) = x.u[0];
+      *reinterpret_cast<uint4*>(p + 16) = x.u[1];
+    }
+  };
+
+  // ---- product
+  f32x4_t acc[TN][TK];
+#pragma unroll
+  for (int a = 0; a < TN; ++a)
+#pragma unroll
+    for (int b = 0; b < TK; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   typedef s16x4_t __attribute__((address_space(3))) * lds_v4;
-  auto trload = [&](const bf16_t* p) {
+  const int swz = wg_swz((lq << 3) + (li >> 2));         // of every row this lane reads
+  const int rowo = (lq * 8 + (li >> 2)) * ROWB + (li & 3) * 8;
+  auto trload = [&](const char* plane, int mc, int f) {  // 16-column tile f of the 32 rows mc: 8 rows of one column for each lane
     union { struct { s16x4_t lo, hi; } s; b16x8_t v; } u;
+    const char* p = plane + mc * (32 * ROWB) + rowo + ((f ^ swz) << 5);
     u.s.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p));
-    u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 4 * WLD));
+    u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 4 * ROWB));
     return u.v;
   };
-  for (long long m = mb; m < me; m += WR) {
-    float gv[4][8];
-    uint2 xq[4];
-    unsigned char xs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long r = m + r0 + 16 * i, rc = r < me ? r : me - 1;
-      const T* row = reinterpret_cast<const T*>(g.G) + rc * g.ldg;
-      const int n = n0 + cv * 8;
-      if (VEC) {
-        ld8<T>(row + (n < g.N ? n : 0), gv[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) gv[i][j] = to_f<T>(row[n + j < g.N ? n + j : 0]);
-      }
-      xq[i] = *reinterpret_cast<const uint2*>(g.X + rc * g.Kp + k0 + cv * 8);
-      xs[i] = g.Xs[rc * g.Sp + kb];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) gv[i][j] = r < me && n + j < g.N ? gv[i][j] : 0.f;
-      if (r >= me) xq[i] = make_uint2(0, 0);
+  if (nst > 0) {
+    fetch(0, 0);
+    commit(0, 0);
+  }
+  wait_vmcnt<0>();
+  lds_barrier();
+  for (int st = 0; st < nst; ++st) {
+    const int buf = st & 1;
+    char* sb = smem + buf * STAGE;
+    if (DMA && me - (mb + (long long)st * R) < R) {       // the last stage is ragged: the rows that its DMA repeated are cleared
+      const int left = (int)(me - (mb + (long long)st * R));
+      for (int i = t + left * (ROWB / 16); i < R * (ROWB / 16); i += NTH) *reinterpret_cast<uint4*>(sb + i * 16) = make_uint4(0, 0, 0, 0);
+      lds_barrier();
     }
-    __syncthreads();                                    // the previous stage has been read
+    if (st + 1 < nst) fetch(st + 1, buf ^ 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int o = (r0 + 16 * i) * WLD + cv * 8;
-      uint4 piece[P];
-      split8<P>(gv[i], piece);
+    for (int mc = 0; mc < R / 32; ++mc) {
+      b16x8_t xf[TK];
 #pragma unroll
-      for (int p = 0; p < P; ++p) *reinterpret_cast<uint4*>(Gs[p] + o) = piece[p];
-      const float s = p8_pow2((int)xs[i] - 127);
-      union { bf2_t h[4]; uint4 u; } x;
-      x.h[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[i].x, s, false);
-      x.h[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[i].x, s, true);
-      x.h[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[i].y, s, false);
-      x.h[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xq[i].y, s, true);
-      *reinterpret_cast<uint4*>(Xl + o) = x.u;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int mc = 0; mc < WR / 32; ++mc) {
-      const int row = (mc * 32 + lq * 8 + (li >> 2)) * WLD + (li & 3) * 4;
-      b16x8_t xf[4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b) xf[b] = trload(Xl + row + (wk * 4 + b) * 16);
+      for (int b = 0; b < TK; ++b) xf[b] = trload(sb + P * PLANE, mc, wk * TK + b);
 #pragma unroll
       for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          const b16x8_t gf = trload(Gs[p] + row + (wn * 4 + a) * 16);
+        for (int a = 0; a < TN; ++a) {
+          const b16x8_t gf = trload(sb + p * PLANE, mc, wn * TN + a);
 #pragma unroll
-          for (int b = 0; b < 4; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(gf, xf[b], acc[a][b], 0, 0, 0);
+          for (int b = 0; b < TK; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[b], gf, acc[a][b], 0, 0, 0);
         }
     }
+    if (st + 1 < nst) commit(st + 1, buf ^ 1);
+    wait_vmcnt<0>();
+    lds_barrier();
   }
+  // a lane holds four neighbouring k of one n
   float* out = g.out + (long long)split * g.plane;
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int a = 0; a < TN; ++a) {
+    const int n = n0 + (wn * TN + a) * 16 + li;
+    if (n >= g.N) continue;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = n0 + (wn * 4 + a) * 16 + lq * 4 + r;
-      if (n >= g.N) continue;
+    for (int b = 0; b < TK; ++b) {
+      const int k = k0 + (wk * TK + b) * 16 + lq * 4;
+      float* p = out + (long long)n * g.ldo + k;
+      f32x4_t v = acc[a][b];
+      if (g.vec && k + 4 <= g.K) {
+        float4 o = make_float4(v[0], v[1], v[2], v[3]);
+        if (g.accumulate) { const float4 q = *reinterpret_cast<const float4*>(p); o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w; }
+        *reinterpret_cast<float4*>(p) = o;
+      } else {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int k = k0 + (wk * 4 + b) * 16 + li;
-        float* p = out + (long long)n * g.ldo + k;
-        if (k < g.K) *p = acc[a][b][r] + (g.accumulate ? *p : 0.f);
+        for (int r = 0; r < 4; ++r)
+          if (k + r < g.K) p[r] = v[r] + (g.accumulate ? p[r] : 0.f);
       }
     }
+  }
 }
 
-// dW (+)= the S partial products, in order
-__global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int S, long long plane, float* dW, long long ldw, int N, int K, int accumulate) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= plane) return;
-  const long long n = i / K;
-  float v = 0.f;
-  for (int s = 0; s < S; ++s) v += part[s * plane + i];
-  float* p = dW + n * ldw + (i - n * K);
-  *p = v + (accumulate ? *p : 0.f);
+// dW (+)= the S partial products, in order: four columns a thread; partial rows hold a multiple of four
+__global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int S, long long plane, float* dW, long long ldw, int N, int K, int accumulate, int vec) {
+  const int q = (K + 3) >> 2;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n = i / q;
+  const int k = (int)(i - n * q) * 4;
+  if (n >= N) return;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < S; ++s) {
+    const float4 x = *reinterpret_cast<const float4*>(part + s * plane + i * 4);
+    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+  }
+  float* p = dW + n * ldw + k;
+  if (vec && k + 4 <= K) {
+    if (accumulate) { const float4 o = *reinterpret_cast<const float4*>(p); v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
+    *reinterpret_cast<float4*>(p) = v;
+  } else {
+    const float e[4] = {v.x, v.y, v.z, v.w};
+    for (int r = 0; r < 4 && k + r < K; ++r) p[r] = e[r] + (accumulate ? p[r] : 0.f);
+  }
 }
 
-struct Split { int S; long long rows; };
-// at least 512 workgroups where the rows allow it (two on each of the 256 compute units), and at least four stages in each
+struct Split { int tile, S; long long rows; };
+// 256 x 256 tiles where at least 192 of them keep the compute units busy, otherwise 128 x 128 with the rows split for at least 256 workgroups, four
+// stages in each
 inline Split split_of(long long M, int N, int K) {
-  const long long tiles = (long long)((N + WT - 1) / WT) * ((K + WT - 1) / WT), stages = (M + WR - 1) / WR;
-  long long S = 512 / tiles;
+  const long long t256 = (long long)((N + 255) / 256) * ((K + 255) / 256), t128 = (long long)((N + 127) / 128) * ((K + 127) / 128), stages = (M + 63) / 64;
+  if (t256 >= 192) return {256, 1, stages * 64};
+  long long S = 256 / t128;
   if (S > stages / 4) S = stages / 4;
   if (S < 1) S = 1;
   const long long per = (stages + S - 1) / S;
-  return {(int)((stages + per - 1) / per), per * WR};
+  return {128, (int)((stages + per - 1) / per), per * 64};
 }
-template <typename T, int P> void run(const Wgrad8Args& g, unsigned blocks, bool vec, hipStream_t s) {
-  if (vec) hipLaunchKernelGGL((wgrad8_kernel<T, P, true>), dim3(blocks), dim3(256), 0, s, g);
-  else hipLaunchKernelGGL((wgrad8_kernel<T, P, false>), dim3(blocks), dim3(256), 0, s, g);
+inline long long part_plane(int N, int K) { return (long long)N * ((K + 3) / 4 * 4); }
+
+template <typename T, int P, bool DMA, bool VEC, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
+  constexpr int LDS = 2 * (P + 1) * (P == 1 ? 64 : 32) * WN * TN * 16 * 2;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&wgrad8_kernel<T, P, DMA, VEC, WN, WK, TN, TK>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (e != hipSuccess) return (int)e;
+  hipLaunchKernelGGL((wgrad8_kernel<T, P, DMA, VEC, WN, WK, TN, TK>), dim3((unsigned)((long long)g.NT * g.KT * S)), dim3(WN * WK * 64), LDS, s, g);
+  SPB_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T, int P, bool DMA, bool VEC> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
+  g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
+  if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
+  return sp.tile == 256 ? launch<T, P, DMA, VEC, 2, 4, 8, 4>(g, sp.S, s) : launch<T, P, DMA, VEC, 2, 2, 4, 4>(g, sp.S, s);
 }
 __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long ldw, int N, int K) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -174,7 +275,7 @@ extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K)
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
   if (M == 0 || N == 0 || K == 0) return 0;
   const Split sp = split_of(M, N, K);
-  return sp.S > 1 ? (long long)sp.S * N * K * 4 : 0;
+  return sp.S > 1 ? (long long)sp.S * part_plane(N, K) * 4 : 0;
 }
 
 extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream_t stream) {
@@ -195,20 +296,21 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
   if (sp.S > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < spb_gemm8_wgrad_bytes(dtype, a->M, a->N, a->K))) return SPB_E_ARG;
   const int es = dtype == SPB_F32 ? 4 : 2;
   const bool vec = a->N % 8 == 0 && ((uintptr_t)a->G & 15) == 0 && (a->ldg * es) % 16 == 0;
-  const long long plane = (long long)a->N * a->K;
-  Wgrad8Args g = {a->G, a->X, a->Xs, sp.S > 1 ? (float*)a->ws : a->dW, a->M, a->ldg, sp.S > 1 ? a->K : a->ldw, sp.S > 1 ? plane : 0, sp.rows, a->N, a->K,
-                  p8_cols(a->K), p8_scales(a->K), (a->N + WT - 1) / WT, (a->K + WT - 1) / WT, sp.S > 1 ? 0 : a->accumulate};
-  const long long blocks = (long long)g.NT * g.KT * sp.S;
-  if (blocks > 0x7fffffffll) return SPB_E_SHAPE;
-  if (dtype == SPB_F32) run<float, 3>(g, (unsigned)blocks, vec, s);
+  const long long plane = part_plane(a->N, a->K);
+  const int outvec = ((uintptr_t)a->dW & 15) == 0 && a->ldw % 4 == 0;
+  const Wgrad8Args g = {a->G, a->X, a->Xs, sp.S > 1 ? (float*)a->ws : a->dW, a->M, a->ldg, sp.S > 1 ? plane / a->N : a->ldw, sp.S > 1 ? plane : 0, sp.rows, a->N, a->K,
+                        p8_cols(a->K), p8_scales(a->K), 0, 0, sp.S > 1 ? 0 : a->accumulate, sp.S > 1 ? 1 : outvec};
+  int e;
+  if (dtype == SPB_F32) e = vec ? run<float, 3, false, true>(g, sp, s) : run<float, 3, false, false>(g, sp, s);
 #ifdef SPB_F16
-  else run<bf16_t, 2>(g, (unsigned)blocks, vec, s);
+  else e = vec ? run<bf16_t, 2, false, true>(g, sp, s) : run<bf16_t, 2, false, false>(g, sp, s);
 #else
-  else run<bf16_t, 1>(g, (unsigned)blocks, vec, s);
+  else e = vec && a->ldg < (1 << 24) ? run<bf16_t, 1, true, true>(g, sp, s) : run<bf16_t, 1, false, false>(g, sp, s);     // 64 rows: 32-bit offsets
 #endif
-  SPB_CHECK_LAUNCH();
+  if (e) return e;
   if (sp.S > 1) {
-    hipLaunchKernelGGL(wgrad8_join_kernel, dim3((unsigned)blocks1), dim3(256), 0, s, (const float*)a->ws, sp.S, plane, a->dW, a->ldw, a->N, a->K, a->accumulate);
+    hipLaunchKernelGGL(wgrad8_join_kernel, dim3((unsigned)((plane / 4 + 255) / 256)), dim3(256), 0, s, (const float*)a->ws, sp.S, plane, a->dW, a->ldw, a->N, a->K,
+                       a->accumulate, outvec);
     SPB_CHECK_LAUNCH();
   }
   return 0;

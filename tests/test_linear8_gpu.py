@@ -180,6 +180,16 @@ def test_product(device, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(3700, 3300, 130), (3329, 3841, 700), (1500, 2000, 1030), (70, 300, 9100), (17, 33, 20000)])
+def test_product_of_every_tile(device, M, N, K, dtype):
+    """256-, 128- and 64-wide tiles with ragged ends, split reductions"""
+    from speedplusbaseline_amd import ops
+    A, (B, _) = ops.quant8(data(M, K, torch.bfloat16, M, scale=0.02)), ops.quant8_weight(data(N, K, torch.float32, N, scale=0.02), transpose=False)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(2)).cuda()
+    check_product(A, B, bias, ops.gemm8(A, B, bias=bias, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("M,N,K", [(1, 40, 256), (5, 17, 1024), (48, 264, 640), (300, 1500, 512), (1024, 1152, 384)])
 def test_product_of_whole_numbers_is_exact(device, M, N, K, dtype):
     """codes -4 .. 4 (scales set by a 448 in a column the other side has 0 in): every sum is a whole number below 2^24, in any order"""
@@ -261,6 +271,17 @@ def test_wgrad(device, M, N, K, layout, dtype):
     out = ops.gemm8_wgrad(G, X8, dW=wide[:, 2:2 + K])
     check_wgrad(G, X8, out, before[:, 2:2 + K])
     assert torch.equal(wide[:, :2].double(), before[:, :2]) and torch.equal(wide[:, 2 + K:].double(), before[:, 2 + K:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(70, 3500, 3600), (200, 3593, 3329), (5000, 136, 700), (9000, 17, 40)])
+def test_wgrad_of_every_tile(device, M, N, K, dtype):
+    """256- and 128-wide tiles with ragged ends, split rows"""
+    from speedplusbaseline_amd import ops
+    G, X8 = data(M, N, dtype, M, scale=1e-3), ops.quant8(data(M, K, torch.bfloat16, N))
+    check_wgrad(G, X8, ops.gemm8_wgrad(G, X8))
+    before = torch.randn(N, K, device="cuda")
+    check_wgrad(G, X8, ops.gemm8_wgrad(G, X8, dW=before.clone()), before.double())
 
 
 def test_wgrad_keeps_all_bits_of_the_gradient(device):
