@@ -12,7 +12,7 @@
 //   * Workgroups walk the rows with a stride, gamma and beta stay in registers, and the next row is requested before this one is summed.
 //   * dgamma / dbeta: a thread keeps its columns' sums in registers over its rows, the groups of a workgroup join through LDS, a workgroup
 //     stores one partial row, and a second launch adds the partial rows in order: no atomics, the same bits in every run.
-#include "common.h"
+#include "vec8.h"
 
 namespace {
 
@@ -20,15 +20,34 @@ constexpr int LN_REG_MAX = 8192;      // longest row held in registers
 constexpr int LN_FWD_WGS = 2048;      // workgroups that walk the rows: eight of 256 threads on each of the 256 compute units
 constexpr int LN_BWD_WGS = 512;       // backward: each stores one partial row of 2 C floats, so fewer of them
 
-// the 8 * NV elements of a row that a thread holds: vectors of 8 (VEC: 16-byte aligned rows and C % 8 == 0) or single elements a group apart
-template <typename T, int TPR, int NV, bool VEC> struct RowRegs {
-  Raw8<T> r[NV];
-  __device__ __forceinline__ void load(const T* row, int C, int lane) {
+// The 8 * NV elements of a row that a thread holds.
+//   VEC (C a multiple of 8): vectors of 8, a group apart, at any alignment.  Vectors in front of number `last` lie inside the row for every thread, those
+//   behind it outside, both the same for the whole launch: only vector `last` is compared with the row's end.
+//   Otherwise single elements a group apart: a wave still reads whole lines.  (Vectors at odd addresses with their row's end shifted or loaded into
+//   place were built and take twice as long: 2351 x 1001, 12 against 6 us.)
+template <int TPR, bool VEC> struct RowEnd {
+  int C, lane, last;
+  __device__ __forceinline__ RowEnd(int C_, int lane_) : C(C_), lane(lane_), last((C_ >> 3) / TPR) {}
+  __device__ __forceinline__ int col(int j, int i) const { return VEC ? (j * TPR + lane) * 8 + i : (j * 8 + i) * TPR + lane; }
+  // f(j, i, true) for the elements of whole vectors, f(j, i, inside) for the others that may be inside
+  template <int NV, typename F> __device__ __forceinline__ void each(F f) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * TPR + lane) * 8;
-      r[j] = ldraw<T>(row + (c < C ? c : 0));
+      if (!VEC || j == last) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f(j, i, VEC ? (j * TPR + lane) * 8 < C : col(j, i) < C);
+      } else if (j < last) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f(j, i, true);
+      }
     }
+  }
+};
+template <typename T, int TPR, int NV, bool VEC> struct RowRegs {
+  Raw8<T> r[NV];
+  __device__ __forceinline__ void load(const T* row, const RowEnd<TPR, VEC>& end) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) r[j] = vec_get<T, 0>(row, end.col(j, 0), end.C);
   }
   __device__ __forceinline__ void get(float v[NV][8]) const {
 #pragma unroll
@@ -37,14 +56,11 @@ template <typename T, int TPR, int NV, bool VEC> struct RowRegs {
 };
 template <typename T, int TPR, int NV> struct RowRegs<T, TPR, NV, false> {
   T e[NV][8];
-  __device__ __forceinline__ void load(const T* row, int C, int lane) {
+  __device__ __forceinline__ void load(const T* row, const RowEnd<TPR, false>& end) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = (j * 8 + i) * TPR + lane;
-        e[j][i] = row[c < C ? c : 0];
-      }
+      for (int i = 0; i < 8; ++i) e[j][i] = row[end.col(j, i) < end.C ? end.col(j, i) : 0];
   }
   __device__ __forceinline__ void get(float v[NV][8]) const {
 #pragma unroll
@@ -53,43 +69,27 @@ template <typename T, int TPR, int NV> struct RowRegs<T, TPR, NV, false> {
       for (int i = 0; i < 8; ++i) v[j][i] = to_f<T>(e[j][i]);
   }
 };
-template <int TPR, bool VEC> __device__ __forceinline__ int ln_col(int j, int i, int lane) {
-  return VEC ? (j * TPR + lane) * 8 + i : (j * 8 + i) * TPR + lane;
-}
-template <int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_param(const float* p, float other, int C, int lane, float v[NV][8]) {
+template <int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_param(const float* p, float other, const RowEnd<TPR, VEC>& end, float v[NV][8]) {
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[j][i] = other;
   if (p == nullptr) return;
-  const bool whole = VEC && ((uintptr_t)p & 15) == 0;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (whole) {
-      const int c = (j * TPR + lane) * 8;
-      ld8<float>(p + (c < C ? c : 0), v[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = ln_col<TPR, VEC>(j, i, lane);
-        v[j][i] = p[c < C ? c : 0];
-      }
-    }
-  }
+  RowRegs<float, TPR, NV, VEC> r;
+  r.load(p, end);
+  r.get(v);
 }
-template <typename T, int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_store(T* row, int C, int lane, const float v[NV][8]) {
+template <typename T, int TPR, int NV, bool VEC> __device__ __forceinline__ void ln_store(T* row, const RowEnd<TPR, VEC>& end, const float v[NV][8]) {
+  if constexpr (VEC) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    if (VEC) {
-      const int c = (j * TPR + lane) * 8;
-      if (c < C) st8<T>(row + c, v[j]);
-    } else {
+    for (int j = 0; j < NV; ++j)
+      if (j <= end.last) vec_put<T, 0>(row, end.col(j, 0), end.C, v[j]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int c = (j * 8 + i) * TPR + lane;
-        if (c < C) row[c] = from_f<T>(v[j][i]);
-      }
-    }
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (end.col(j, i) < end.C) row[end.col(j, i)] = from_f<T>(v[j][i]);
   }
 }
 
@@ -117,50 +117,38 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const spb_layernorm_args_t 
   __shared__ float red[4][4];
   const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
   const int C = a.C;
+  const RowEnd<TPR, VEC> end(C, lane);
   const float inv = 1.f / (float)C;
   const T* X = reinterpret_cast<const T*>(a.X);
   T* Y = reinterpret_cast<T*>(a.Y);
   const long long step = (long long)gridDim.x * GR;
   long long m = (long long)blockIdx.x * GR + grp;
   RowRegs<T, TPR, NV, VEC> cur, nxt;
-  cur.load(X + (m < a.M ? m : a.M - 1) * a.ldx, C, lane);
+  cur.load(X + (m < a.M ? m : a.M - 1) * a.ldx, end);
   float gm[NV][8], bt[NV][8];
-  ln_param<TPR, NV, VEC>(a.gamma, 1.f, C, lane, gm);
-  ln_param<TPR, NV, VEC>(a.beta, 0.f, C, lane, bt);
-  // TPR 256: m is the same in the whole workgroup, so is the trip count; the other groups of a wave may end a trip apart (no barrier there,
-  // and the DPP sums of a group read its own lanes only -- the loop runs until the last group of the WAVE is done)
-  const long long first = TPR == 256 ? m : (long long)blockIdx.x * GR + (threadIdx.x >> 6) * (64 / (TPR < 64 ? TPR : 64));
+  ln_param<TPR, NV, VEC>(a.gamma, 1.f, end, gm);
+  ln_param<TPR, NV, VEC>(a.beta, 0.f, end, bt);
+  // a group's row is past the end for whole groups: the sums of a group read its own lanes only, and with TPR 256 (barriers) the group is the workgroup
   int flip = 0;
-  for (long long base = first; base < a.M; base += step, m += step, flip ^= 2) {
+  for (; m < a.M; m += step, flip ^= 2) {
     const long long mn = m + step;
-    nxt.load(X + (mn < a.M ? mn : a.M - 1) * a.ldx, C, lane);
+    nxt.load(X + (mn < a.M ? mn : m) * a.ldx, end);
     float v[NV][8];
     cur.get(v);
     float s[1] = {0.f};
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[0] += ln_col<TPR, VEC>(j, i, lane) < C ? v[j][i] : 0.f;
+    end.template each<NV>([&](int j, int i, bool in) { s[0] += in ? v[j][i] : 0.f; });
     group_sum<TPR, 1>(s, red[flip]);
     const float mean = s[0] * inv;
     float q[1] = {0.f};
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[j][i] -= mean;
-        q[0] += ln_col<TPR, VEC>(j, i, lane) < C ? v[j][i] * v[j][i] : 0.f;
-      }
+    end.template each<NV>([&](int j, int i, bool in) {
+      v[j][i] = in ? v[j][i] - mean : 0.f;
+      q[0] += v[j][i] * v[j][i];
+    });
     group_sum<TPR, 1>(q, red[flip + 1]);
     const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = v[j][i] * rstd * gm[j][i] + bt[j][i];
-    if (m < a.M) {
-      ln_store<T, TPR, NV, VEC>(Y + m * a.ldy, C, lane, v);
-      if (lane == 0) { a.mean[m] = mean; a.rstd[m] = rstd; }
-    }
+    end.template each<NV>([&](int j, int i, bool) { v[j][i] = v[j][i] * rstd * gm[j][i] + bt[j][i]; });
+    ln_store<T, TPR, NV, VEC>(Y + m * a.ldy, end, v);
+    if (lane == 0) { a.mean[m] = mean; a.rstd[m] = rstd; }
     cur = nxt;
   }
 }
@@ -199,6 +187,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t 
   __shared__ float join[SUMS && GR > 1 ? GR * TPR * NV * 8 : 1];
   const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
   const int C = a.C;
+  const RowEnd<TPR, VEC> end(C, lane);
   const float inv = 1.f / (float)C;
   const T* X = reinterpret_cast<const T*>(a.X);
   const T* G = reinterpret_cast<const T*>(a.G);
@@ -209,45 +198,34 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t 
   float cm, cr, nm, nr;
   {
     const long long mc = m < a.M ? m : a.M - 1;
-    cx.load(X + mc * a.ldx, C, lane); cg.load(G + mc * a.ldg, C, lane);
+    cx.load(X + mc * a.ldx, end); cg.load(G + mc * a.ldg, end);
     cm = a.mean[mc]; cr = a.rstd[mc];
   }
   float gm[NV][8], dg[NV][8], db[NV][8];
-  ln_param<TPR, NV, VEC>(a.gamma, 1.f, C, lane, gm);
+  ln_param<TPR, NV, VEC>(a.gamma, 1.f, end, gm);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) { dg[j][i] = 0.f; db[j][i] = 0.f; }
-  const long long first = TPR == 256 ? m : (long long)blockIdx.x * GR + (threadIdx.x >> 6) * (64 / (TPR < 64 ? TPR : 64));
   int flip = 0;
-  for (long long base = first; base < a.M; base += step, m += step, flip ^= 1) {
-    const long long mn = m + step, mc = mn < a.M ? mn : a.M - 1;
-    nx.load(X + mc * a.ldx, C, lane); ng.load(G + mc * a.ldg, C, lane);
+  for (; m < a.M; m += step, flip ^= 1) {      // whole groups leave: see the forward kernel
+    const long long mn = m + step, mc = mn < a.M ? mn : m;
+    nx.load(X + mc * a.ldx, end); ng.load(G + mc * a.ldg, end);
     nm = a.mean[mc]; nr = a.rstd[mc];
     float x[NV][8], g[NV][8];
     cx.get(x); cg.get(g);
-    const bool row = m < a.M;
     float s[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = row && ln_col<TPR, VEC>(j, i, lane) < C;
-        x[j][i] = in ? (x[j][i] - cm) * cr : 0.f;           // xh
-        g[j][i] = in ? g[j][i] : 0.f;
-        if (SUMS) { dg[j][i] += g[j][i] * x[j][i]; db[j][i] += g[j][i]; }
-        g[j][i] *= gm[j][i];                                 // h
-        s[0] += g[j][i]; s[1] += g[j][i] * x[j][i];
-      }
+    end.template each<NV>([&](int j, int i, bool in) {
+      x[j][i] = in ? (x[j][i] - cm) * cr : 0.f;             // xh
+      g[j][i] = in ? g[j][i] : 0.f;
+      if (SUMS) { dg[j][i] += g[j][i] * x[j][i]; db[j][i] += g[j][i]; }
+      g[j][i] *= gm[j][i];                                   // h
+      s[0] += g[j][i]; s[1] += g[j][i] * x[j][i];
+    });
     group_sum<TPR, 2>(s, red[flip]);
     const float s1 = s[0] * inv, s2 = s[1] * inv;
-    if (row) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[j][i] = cr * (g[j][i] - s1 - x[j][i] * s2);
-      ln_store<T, TPR, NV, VEC>(D + m * a.ldy, C, lane, g);
-    }
+    end.template each<NV>([&](int j, int i, bool) { g[j][i] = cr * (g[j][i] - s1 - x[j][i] * s2); });
+    ln_store<T, TPR, NV, VEC>(D + m * a.ldy, end, g);
     cx = nx; cg = ng; cm = nm; cr = nr;
   }
   if (SUMS) {
@@ -259,7 +237,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t 
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) join[grp * (TPR * NV * 8) + ln_col<TPR, VEC>(j, i, lane)] = half ? db[j][i] : dg[j][i];
+          for (int i = 0; i < 8; ++i) join[grp * (TPR * NV * 8) + end.col(j, i)] = half ? db[j][i] : dg[j][i];
         __syncthreads();
         for (int c = threadIdx.x; c < C; c += 256) {
           float v = 0.f;
@@ -272,7 +250,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t 
         for (int j = 0; j < NV; ++j)
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int c = ln_col<TPR, VEC>(j, i, lane);
+            const int c = end.col(j, i);
             if (c < C) out[half * C + c] = half ? db[j][i] : dg[j][i];
           }
       }
@@ -364,8 +342,6 @@ inline int ln_bwd_parts(long long M, int C) {
   const long long wgs = (M + 256 / ln_shape(C).tpr - 1) / (256 / ln_shape(C).tpr);
   return (int)(wgs < LN_BWD_WGS ? (wgs > 0 ? wgs : 1) : LN_BWD_WGS);
 }
-inline bool aligned16(const void* p, long long ld, int es) { return ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0; }
-
 template <typename T, bool VEC> void launch_fwd(const spb_layernorm_args_t& a, hipStream_t s) {
   const LnShape sh = ln_shape(a.C);
   const long long gr = 256 / sh.tpr, need = (a.M + gr - 1) / gr;
@@ -385,6 +361,27 @@ template <typename T, bool VEC, bool SUMS> void launch_bwd(const spb_layernorm_a
   else { if (sh.nv == 1) LN_B(256, 1); else if (sh.nv == 2) LN_B(256, 2); else LN_B(256, 4); }
 #undef LN_B
 }
+template <typename T> void run_fwd(const spb_layernorm_args_t& a, hipStream_t s) {
+  if (a.C > LN_REG_MAX) {
+    hipLaunchKernelGGL((ln_fwd_long<T>), dim3((unsigned)(a.M < LN_FWD_WGS ? a.M : LN_FWD_WGS)), dim3(256), 0, s, a);
+    return;
+  }
+  if (a.C % 8 == 0) launch_fwd<T, true>(a, s); else launch_fwd<T, false>(a, s);
+}
+// returns the number of partial rows
+template <typename T> int run_bwd(const spb_layernorm_args_t& a, bool sums, hipStream_t s) {
+  int P = ln_bwd_parts(a.M, a.C);
+  if (a.C > LN_REG_MAX) {
+    const long long rows = (a.M + P - 1) / P;
+    P = (int)((a.M + rows - 1) / rows);             // ranges that hold a row
+    if (sums) hipLaunchKernelGGL((ln_bwd_cols<T>), dim3((unsigned)((a.C + 255) / 256), (unsigned)P), dim3(256), 0, s, a, rows);
+    hipLaunchKernelGGL((ln_bwd_long<T>), dim3((unsigned)(a.M < LN_FWD_WGS ? a.M : LN_FWD_WGS)), dim3(256), 0, s, a);
+    return P;
+  }
+  if (sums) { if (a.C % 8 == 0) launch_bwd<T, true, true>(a, s); else launch_bwd<T, false, true>(a, s); }
+  else { if (a.C % 8 == 0) launch_bwd<T, true, false>(a, s); else launch_bwd<T, false, false>(a, s); }
+  return P;
+}
 
 int check_args(int dtype, const spb_layernorm_args_t* a, bool bwd) {
   if (dtype != SPB_F32 && dtype != SPB_BF16) return SPB_E_ARG;
@@ -402,17 +399,7 @@ extern "C" int spb_layernorm_fwd(int dtype, const spb_layernorm_args_t* a, spb_s
   if (bad) return bad;
   if (a->M == 0) return 0;
   hipStream_t s = (hipStream_t)stream;
-  const int es = dtype == SPB_F32 ? 4 : 2;
-  const bool vec = a->C % 8 == 0 && aligned16(a->X, a->ldx, es) && aligned16(a->Y, a->ldy, es);
-  if (a->C > LN_REG_MAX) {
-    const dim3 grid((unsigned)(a->M < LN_FWD_WGS ? a->M : LN_FWD_WGS));
-    if (dtype == SPB_F32) hipLaunchKernelGGL((ln_fwd_long<float>), grid, dim3(256), 0, s, *a);
-    else hipLaunchKernelGGL((ln_fwd_long<bf16_t>), grid, dim3(256), 0, s, *a);
-  } else if (dtype == SPB_F32) {
-    if (vec) launch_fwd<float, true>(*a, s); else launch_fwd<float, false>(*a, s);
-  } else {
-    if (vec) launch_fwd<bf16_t, true>(*a, s); else launch_fwd<bf16_t, false>(*a, s);
-  }
+  if (dtype == SPB_F32) run_fwd<float>(*a, s); else run_fwd<bf16_t>(*a, s);
   SPB_CHECK_LAUNCH();
   return 0;
 }
@@ -429,29 +416,8 @@ extern "C" int spb_layernorm_bwd(int dtype, const spb_layernorm_args_t* a, spb_s
   if (a->M == 0 && (!sums || a->accumulate)) return 0;
   if (sums && a->M > 0 && (!a->part || a->part_cap < spb_layernorm_bwd_floats(a->M, a->C))) return SPB_E_ARG;
   hipStream_t s = (hipStream_t)stream;
-  const int es = dtype == SPB_F32 ? 4 : 2;
-  const bool vec = a->C % 8 == 0 && aligned16(a->X, a->ldx, es) && aligned16(a->G, a->ldg, es) && aligned16(a->Y, a->ldy, es);
-  int P = ln_bwd_parts(a->M, a->C);
-  if (a->M == 0) {
-    P = 0;                                          // no rows: the join writes zeros
-  } else if (a->C > LN_REG_MAX) {
-    const long long rows = (a->M + P - 1) / P;
-    P = (int)((a->M + rows - 1) / rows);            // ranges that hold a row
-    const dim3 cols((unsigned)((a->C + 255) / 256), (unsigned)P), grid((unsigned)(a->M < LN_FWD_WGS ? a->M : LN_FWD_WGS));
-    if (dtype == SPB_F32) {
-      if (sums) hipLaunchKernelGGL((ln_bwd_cols<float>), cols, dim3(256), 0, s, *a, rows);
-      hipLaunchKernelGGL((ln_bwd_long<float>), grid, dim3(256), 0, s, *a);
-    } else {
-      if (sums) hipLaunchKernelGGL((ln_bwd_cols<bf16_t>), cols, dim3(256), 0, s, *a, rows);
-      hipLaunchKernelGGL((ln_bwd_long<bf16_t>), grid, dim3(256), 0, s, *a);
-    }
-  } else if (dtype == SPB_F32) {
-    if (sums) { if (vec) launch_bwd<float, true, true>(*a, s); else launch_bwd<float, false, true>(*a, s); }
-    else { if (vec) launch_bwd<float, true, false>(*a, s); else launch_bwd<float, false, false>(*a, s); }
-  } else {
-    if (sums) { if (vec) launch_bwd<bf16_t, true, true>(*a, s); else launch_bwd<bf16_t, false, true>(*a, s); }
-    else { if (vec) launch_bwd<bf16_t, true, false>(*a, s); else launch_bwd<bf16_t, false, false>(*a, s); }
-  }
+  int P = 0;                                        // no rows: the join writes zeros
+  if (a->M > 0) P = dtype == SPB_F32 ? run_bwd<float>(*a, sums, s) : run_bwd<bf16_t>(*a, sums, s);
   SPB_CHECK_LAUNCH();
   if (sums) {
     hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((2ll * a->C + 63) / 64)), dim3(LN_JOIN * 64), 0, s, a->part, P, a->C, a->dgamma, a->dbeta, a->accumulate);

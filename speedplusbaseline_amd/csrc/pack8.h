@@ -1,6 +1,6 @@
 // The packed 8-bit format of include/spb_hip.h ("8-bit packing"): what its writers and readers share.
 #pragma once
-#include "common.h"
+#include "vec8.h"
 
 #define P8_BLOCK 128                  // columns (and, for weights, rows) that share a scale
 #define P8_E_LOW (-110)               // smallest / largest exponent of a scale: every value code * 2^e is then a normal bfloat16

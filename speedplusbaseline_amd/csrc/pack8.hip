@@ -16,48 +16,57 @@ __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, spb_dpp_f<0xB1>(v)); v = fmaxf(v, spb_dpp_f<0x4E>(v)); v = fmaxf(v, spb_dpp_f<0x141>(v)); v = fmaxf(v, spb_dpp_f<0x140>(v));
   return v;
 }
-// 8 elements from column c on (zeros behind K).  VEC: 16-byte aligned rows and K % 8 == 0.
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, int c, int K, float v[8]) {
-  if (VEC) {
-    float t[8];
-    ld8<T>(row + (c < K ? c : 0), t);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c < K ? t[i] : 0.f;
-  } else {
+// 8 elements from column c on, zeros behind K (MODE: vec8.h)
+template <typename T, int MODE> __device__ __forceinline__ void load8(const T* row, int c, int K, float v[8]) {
+  if constexpr (MODE == 2) {
     T t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = row[c + i < K ? c + i : 0];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f<T>(t[i]) : 0.f;
+  } else {
+    Raw8<T> r = vec_get<T, MODE>(row, c, K);
+    vec_place<T, MODE>(r, c, K);
+    cvt8(r, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + (MODE == 0 ? 0 : i) < K ? v[i] : 0.f;
   }
 }
 // The f32 value is what is rounded, in both forms: without the empty asm the compiler may fold a product into its conversion to half (one rounding
-// instead of two) in one of them, and a result would depend on its tensor's alignment.
-template <typename T, bool VEC> __device__ __forceinline__ void store8(T* row, int c, int K, float v[8]) {
+// instead of two) in one of them, and a result would depend on its row's length.
+template <typename T, int MODE> __device__ __forceinline__ void store8(T* row, int c, int K, float v[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) asm("" : "+v"(v[i]));
-  if (VEC) {
-    if (c < K) st8<T>(row + c, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < K) row[c + i] = from_f<T>(v[i]);
-  }
+  vec_put<T, MODE>(row, c, K, v);
 }
 
-// act'(x) and act(x) in f32.  ACT 0: none (plain packing).
+// act(x) and act'(x) in f32 (ACT 0: none, plain packing), from one exponential and one reciprocal each: with the library's erff, tanhf, expf and the exact
+// division both passes were bound by vector instructions (16384 x 4096 bfloat16: 88 / 102 us).
+//   sigmoid    s = 1 / (1 + e^-x);   silu = x s,  silu' = s (1 + x (1 - s))
+//   gelu tanh  (1 + tanh u) / 2 = sigmoid(2 u),  u = sqrt(2 / pi) (x + 0.044715 x^3)
+//   gelu       Phi(x) = 1 - Q or Q, Q = erfc(|x| / sqrt 2) / 2 = t (a1 + t (a2 + ...)) e^(-x^2 / 2) / 2, t = 1 / (1 + p |x| / sqrt 2): Abramowitz and Stegun
+//              7.1.26, |error of erf| <= 1.5e-7; the density's exponential is the same one
+__device__ __forceinline__ float p8_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+__device__ __forceinline__ float p8_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + p8_exp(-x)); }
+__device__ __forceinline__ float p8_phi(float x, float& e) {      // Phi(x); e = e^(-x^2 / 2)
+  const float a = fabsf(x);
+  e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.23164189f, 1.f));
+  const float q = fmaf(fmaf(fmaf(fmaf(0.5307027145f, t, -0.7265760135f), t, 0.7107068705f), t, -0.142248368f), t, 0.127414796f) * t * e;
+  return x < 0.f ? q : 1.f - q;
+}
 template <int ACT> __device__ __forceinline__ float act8(float x) {
-  if (ACT == SPB_ACT_SILU) return x / (1.f + expf(-x));
-  if (ACT == SPB_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678f));
-  if (ACT == SPB_ACT_GELU_TANH) return 0.5f * x * (1.f + tanhf(0.79788456f * (x + 0.044715f * x * x * x)));
-  return x;
+  float e;
+  if (ACT == SPB_ACT_SILU) return x * p8_sigmoid(x);
+  if (ACT == SPB_ACT_GELU) return x * p8_phi(x, e);
+  return x * p8_sigmoid(1.59576912f * fmaf(0.044715f * x, x * x, x));
 }
 template <int ACT> __device__ __forceinline__ float act8_slope(float x) {
-  if (ACT == SPB_ACT_SILU) { const float s = 1.f / (1.f + expf(-x)); return s * (1.f + x * (1.f - s)); }
-  if (ACT == SPB_ACT_GELU) return 0.5f * (1.f + erff(x * 0.70710678f)) + x * 0.39894228f * expf(-0.5f * x * x);
-  x = x > 16.f ? 16.f : (x < -16.f ? -16.f : x);       // 1 - t^2 is 0 from there on; x * x would overflow in 0 * inf.  NaN stays NaN.
-  const float t = tanhf(0.79788456f * (x + 0.044715f * x * x * x));
-  return 0.5f * (1.f + t) + 0.5f * x * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * x * x);
+  if (ACT == SPB_ACT_SILU) { const float s = p8_sigmoid(x); return s * fmaf(x, 1.f - s, 1.f); }
+  if (ACT == SPB_ACT_GELU) { float e; const float p = p8_phi(x, e); return fmaf(x * 0.39894228f, e, p); }
+  x = x > 16.f ? 16.f : (x < -16.f ? -16.f : x);       // s (1 - s) is 0 from there on; x * x would overflow in 0 * inf.  NaN stays NaN.
+  const float s = p8_sigmoid(1.59576912f * fmaf(0.044715f * x, x * x, x));
+  return s * fmaf(x * (1.f - s), 1.59576912f * fmaf(0.134145f * x, x, 1.f), 1.f);
 }
 
 struct RowArgs {
@@ -66,7 +75,7 @@ struct RowArgs {
   unsigned blocks;      // M * KB
   int K, KB, Kp, Sp;
 };
-template <typename T, bool VEC, int ACT>
+template <typename T, int MODE, int ACT>
 __global__ __launch_bounds__(256) void pack8_rows_kernel(const RowArgs a) {
   const unsigned u = blockIdx.x * 16 + (threadIdx.x >> 4);
   const int l = threadIdx.x & 15;
@@ -74,7 +83,7 @@ __global__ __launch_bounds__(256) void pack8_rows_kernel(const RowArgs a) {
   const unsigned m = u / (unsigned)a.KB;
   const int kb = (int)(u - m * (unsigned)a.KB), c = kb * P8_BLOCK + l * 8;
   float v[8];
-  load8<T, VEC>(reinterpret_cast<const T*>(a.X) + (long long)m * a.ldx, c, a.K, v);
+  load8<T, MODE>(reinterpret_cast<const T*>(a.X) + (long long)m * a.ldx, c, a.K, v);
   float top = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = fmaxf(top, p8_finite_abs(v[i]));
@@ -87,7 +96,7 @@ __global__ __launch_bounds__(256) void pack8_rows_kernel(const RowArgs a) {
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = act8<ACT>(v[i]);
-    store8<T, VEC>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, y);
+    store8<T, MODE>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, y);
   }
 }
 
@@ -98,7 +107,7 @@ struct UnpackArgs {
   unsigned vecs;        // M * V
   int K, V, Kp, Sp, shift;
 };
-template <typename T, bool VEC, int ACT>
+template <typename T, int MODE, int ACT>
 __global__ __launch_bounds__(256) void unpack8_kernel(const UnpackArgs a) {
   const unsigned u = blockIdx.x * 256 + threadIdx.x;
   if (u >= a.vecs) return;
@@ -110,32 +119,39 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const UnpackArgs a) {
   p8_decode8(q, s, v);
   if (ACT != 0) {
     float g[8];
-    load8<T, VEC>(reinterpret_cast<const T*>(a.G) + (long long)m * a.ldg, c, a.K, g);
+    load8<T, MODE>(reinterpret_cast<const T*>(a.G) + (long long)m * a.ldg, c, a.K, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = g[i] * act8_slope<ACT>(v[i]);
   }
-  store8<T, VEC>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, v);
+  store8<T, MODE>(reinterpret_cast<T*>(a.Y) + (long long)m * a.ldy, c, a.K, v);
 }
 
-// a 128 x 128 block a workgroup: 16 lanes hold 128 columns of a row, 16 rows at a time.  The transposed codes go through LDS (rows of 144 bytes:
-// 16-byte reads, and the 4-byte bank of a byte column moves with its row).
+// a 128 x 128 block a workgroup: 16 lanes hold 128 columns, a thread 8 columns of 8 neighbouring rows, whose codes it transposes in registers: the 8 codes of a
+// column go to LDS as 8 bytes (rows of 136 bytes: neighbouring columns are two banks apart) and come back as 16.
+// byte j of a[i] becomes byte i of t[j]
+__device__ __forceinline__ void p8_transpose4(const unsigned a[4], unsigned t[4]) {
+  const unsigned x0 = __builtin_amdgcn_perm(a[1], a[0], 0x05010400u), x1 = __builtin_amdgcn_perm(a[1], a[0], 0x07030602u);
+  const unsigned y0 = __builtin_amdgcn_perm(a[3], a[2], 0x05010400u), y1 = __builtin_amdgcn_perm(a[3], a[2], 0x07030602u);
+  t[0] = __builtin_amdgcn_perm(y0, x0, 0x05040100u); t[1] = __builtin_amdgcn_perm(y0, x0, 0x07060302u);
+  t[2] = __builtin_amdgcn_perm(y1, x1, 0x05040100u); t[3] = __builtin_amdgcn_perm(y1, x1, 0x07060302u);
+}
 struct WeightArgs {
   const void* W; unsigned char* Q; unsigned char* S; unsigned char* QT; unsigned char* ST;
   long long ldw;
   int N, K, NB, KB, Kp, Sp, Np, SpT;
 };
-template <typename T, bool VEC>
+template <typename T, int MODE>
 __global__ __launch_bounds__(256) void pack8_weight_kernel(const WeightArgs a) {
-  constexpr int LD = 144;
+  constexpr int LD = 136;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) unsigned char tile[128 * LD];     // [column][row]
   const int nb = blockIdx.x / a.KB, kb = blockIdx.x - nb * a.KB;
-  const int l = threadIdx.x & 15, r0 = threadIdx.x >> 4, c = kb * P8_BLOCK + l * 8;
+  const int l = threadIdx.x & 15, r0 = (threadIdx.x >> 4) * 8, c = kb * P8_BLOCK + l * 8;
   float v[8][8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int n = nb * P8_BLOCK + r0 + 16 * i;
-    load8<T, VEC>(reinterpret_cast<const T*>(a.W) + (long long)(n < a.N ? n : 0) * a.ldw, c, a.K, v[i]);
+    const int n = nb * P8_BLOCK + r0 + i;
+    load8<T, MODE>(reinterpret_cast<const T*>(a.W) + (long long)(n < a.N ? n : 0) * a.ldw, c, a.K, v[i]);
     if (n >= a.N) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
@@ -152,14 +168,24 @@ __global__ __launch_bounds__(256) void pack8_weight_kernel(const WeightArgs a) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
   const int e = p8_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  uint2 q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int r = r0 + 16 * i, n = nb * P8_BLOCK + r;
-    const uint2 q = p8_encode8(v[i], e);
-    if (n < a.N) *reinterpret_cast<uint2*>(a.Q + (size_t)n * a.Kp + c) = q;
-    if (a.QT) {
+    const int n = nb * P8_BLOCK + r0 + i;
+    q[i] = p8_encode8(v[i], e);
+    if (n < a.N) *reinterpret_cast<uint2*>(a.Q + (size_t)n * a.Kp + c) = q[i];
+  }
+  if (a.QT) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) tile[(l * 8 + j) * LD + r] = (unsigned char)((j < 4 ? q.x >> (8 * j) : q.y >> (8 * (j - 4))) & 255u);
+    for (int h = 0; h < 2; ++h) {                        // columns 4 h .. 4 h + 3: two 4 x 4 byte transposes
+      unsigned lo[4], hi[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { lo[i] = h ? q[i].y : q[i].x; hi[i] = h ? q[i + 4].y : q[i + 4].x; }
+      unsigned tl[4], th[4];
+      p8_transpose4(lo, tl);
+      p8_transpose4(hi, th);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(tile + (l * 8 + h * 4 + j) * LD + r0) = make_uint2(tl[j], th[j]);
     }
   }
   if (threadIdx.x == 0) a.S[(size_t)nb * a.Sp + kb] = (unsigned char)(e + 127);
@@ -172,47 +198,43 @@ __global__ __launch_bounds__(256) void pack8_weight_kernel(const WeightArgs a) {
     for (int i = 0; i < 4; ++i) {
       const int idx = threadIdx.x + 256 * i, col = idx >> 3, part = idx & 7, k = kb * P8_BLOCK + col;
       if (k < a.K)
-        *reinterpret_cast<uint4*>(a.QT + (size_t)k * a.Np + nb * P8_BLOCK + part * 16) = *reinterpret_cast<const uint4*>(tile + col * LD + part * 16);
+      {
+        const uint2 u0 = *reinterpret_cast<const uint2*>(tile + col * LD + part * 16), u1 = *reinterpret_cast<const uint2*>(tile + col * LD + part * 16 + 8);
+        *reinterpret_cast<uint4*>(a.QT + (size_t)k * a.Np + nb * P8_BLOCK + part * 16) = make_uint4(u0.x, u0.y, u1.x, u1.y);
+      }
     }
   }
 }
 
-inline bool rows_aligned(const void* p, long long ld, int es, int K) { return K % 8 == 0 && ((uintptr_t)p & 15) == 0 && (ld * es) % 16 == 0; }
 inline bool bad_codes(const void* q, const void* s) { return !q || !s || ((uintptr_t)q & 15) || ((uintptr_t)s & 3); }
 inline bool bad_dtype(int d) { return d != SPB_F32 && d != SPB_BF16; }
 
+// one instance for each type and row length (MODE)
+#define P8_LAUNCH(kernel, grid, ...)                                                                                                        \
+  do {                                                                                                                                      \
+    const int mode_ = vec_mode(a.K);                                                                                                        \
+    if (dtype == SPB_F32) {                                                                                                                 \
+      if (mode_ == 0) hipLaunchKernelGGL((kernel<float, 0, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                      \
+      else if (mode_ == 1) hipLaunchKernelGGL((kernel<float, 1, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                 \
+      else hipLaunchKernelGGL((kernel<float, 2, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                                 \
+    } else {                                                                                                                                \
+      if (mode_ == 0) hipLaunchKernelGGL((kernel<bf16_t, 0, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                     \
+      else if (mode_ == 1) hipLaunchKernelGGL((kernel<bf16_t, 1, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                \
+      else hipLaunchKernelGGL((kernel<bf16_t, 2, ##__VA_ARGS__>), grid, dim3(256), 0, s, a);                                                \
+    }                                                                                                                                       \
+    SPB_CHECK_LAUNCH();                                                                                                                     \
+  } while (0)
+
 template <int ACT> int pack_rows(int dtype, RowArgs a, long long M, hipStream_t s) {
-  const int es = dtype == SPB_F32 ? 4 : 2;
-  bool vec = rows_aligned(a.X, a.ldx, es, a.K);
-  if (ACT != 0) vec = vec && rows_aligned(a.Y, a.ldy, es, a.K);
   if (M * a.KB > 0xfffffff0ll) return SPB_E_SHAPE;
   a.blocks = (unsigned)(M * a.KB);
-  const dim3 grid(a.blocks / 16 + (a.blocks % 16 ? 1 : 0));
-  if (dtype == SPB_F32) {
-    if (vec) hipLaunchKernelGGL((pack8_rows_kernel<float, true, ACT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((pack8_rows_kernel<float, false, ACT>), grid, dim3(256), 0, s, a);
-  } else {
-    if (vec) hipLaunchKernelGGL((pack8_rows_kernel<bf16_t, true, ACT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((pack8_rows_kernel<bf16_t, false, ACT>), grid, dim3(256), 0, s, a);
-  }
-  SPB_CHECK_LAUNCH();
+  P8_LAUNCH(pack8_rows_kernel, dim3(a.blocks / 16 + (a.blocks % 16 ? 1 : 0)), ACT);
   return 0;
 }
 template <int ACT> int unpack(int dtype, UnpackArgs a, long long M, hipStream_t s) {
-  const int es = dtype == SPB_F32 ? 4 : 2;
-  bool vec = rows_aligned(a.Y, a.ldy, es, a.K);
-  if (ACT != 0) vec = vec && rows_aligned(a.G, a.ldg, es, a.K);
   if (M * a.V > 0xfffffff0ll) return SPB_E_SHAPE;
   a.vecs = (unsigned)(M * a.V);
-  const dim3 grid(a.vecs / 256 + (a.vecs % 256 ? 1 : 0));
-  if (dtype == SPB_F32) {
-    if (vec) hipLaunchKernelGGL((unpack8_kernel<float, true, ACT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((unpack8_kernel<float, false, ACT>), grid, dim3(256), 0, s, a);
-  } else {
-    if (vec) hipLaunchKernelGGL((unpack8_kernel<bf16_t, true, ACT>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((unpack8_kernel<bf16_t, false, ACT>), grid, dim3(256), 0, s, a);
-  }
-  SPB_CHECK_LAUNCH();
+  P8_LAUNCH(unpack8_kernel, dim3(a.vecs / 256 + (a.vecs % 256 ? 1 : 0)), ACT);
   return 0;
 }
 
@@ -234,17 +256,8 @@ extern "C" int spb_pack8_weight(int dtype, const void* W, long long ldw, int N, 
   if (!W || bad_codes(codes, scales) || (codesT != nullptr) != (scalesT != nullptr) || (codesT && bad_codes(codesT, scalesT))) return SPB_E_ARG;
   const WeightArgs a = {W, codes, scales, codesT, scalesT, ldw, N, K, (N + 127) / 128, (K + 127) / 128, p8_cols(K), p8_scales(K), p8_cols(N), p8_scales(N)};
   if ((long long)a.NB * a.KB > 0x7fffffffll) return SPB_E_SHAPE;
-  const bool vec = rows_aligned(W, ldw, dtype == SPB_F32 ? 4 : 2, K);
-  const dim3 grid((unsigned)(a.NB * a.KB));
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == SPB_F32) {
-    if (vec) hipLaunchKernelGGL((pack8_weight_kernel<float, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((pack8_weight_kernel<float, false>), grid, dim3(256), 0, s, a);
-  } else {
-    if (vec) hipLaunchKernelGGL((pack8_weight_kernel<bf16_t, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((pack8_weight_kernel<bf16_t, false>), grid, dim3(256), 0, s, a);
-  }
-  SPB_CHECK_LAUNCH();
+  P8_LAUNCH(pack8_weight_kernel, dim3((unsigned)(a.NB * a.KB)));
   return 0;
 }
 

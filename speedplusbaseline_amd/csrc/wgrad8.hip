@@ -46,8 +46,9 @@ template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 
 }
 __device__ __forceinline__ int wg_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-// WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  DMA: G straight to LDS (P == 1, aligned rows); VEC: aligned rows through registers
-template <typename T, int P, bool DMA, bool VEC, int WN, int WK, int TN, int TK>
+// WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  DMA: G straight to LDS (P == 1, 16-byte aligned rows, MODE 0); otherwise through
+// registers (MODE: vec8.h)
+template <typename T, int P, bool DMA, int MODE, int WN, int WK, int TN, int TK>
 __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g) {
   constexpr int TW = WN * TN * 16, NW = WN * WK, NTH = NW * 64;
   static_assert(WK * TK * 16 == TW && (!DMA || P == 1), "square tiles; DMA does not split");
@@ -92,13 +93,13 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
         const int r = gr + i * GRW, rc = r < last ? r : last;
         const T* row = reinterpret_cast<const T*>(g.G) + (m + rc) * g.ldg;
         const int n = n0 + gc;
-        if (VEC) {
-          graw[i] = ldraw<T>(row + (n < g.N ? n : 0));
-        } else {
+        if constexpr (MODE == 2) {
           T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = row[n + j < g.N ? n + j : 0];
           __builtin_memcpy(&graw[i], e, sizeof(graw[i]));
+        } else {
+          graw[i] = vec_get<T, MODE>(row, n, g.N);
         }
       }
     }
@@ -117,6 +118,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
       for (int i = 0; i < GP; ++i) {
         const int r = gr + i * GRW;
         float v[8];
+        if constexpr (MODE == 1) vec_place<T, MODE>(graw[i], n0 + gc, g.N);
         cvt8(graw[i], v);
         uint4 piece[P];
         split8<P>(v, piece);
@@ -239,9 +241,10 @@ __global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int
 struct Split { int tile, S; long long rows; };
 // 256 x 256 tiles where at least 192 of them keep the compute units busy, otherwise 128 x 128 with the rows split for at least 256 workgroups, four
 // stages in each
-inline Split split_of(long long M, int N, int K) {
+// (f32 gradients with rows that end inside a vector: three pieces and the shift into place do not fit the registers of the large tile)
+inline Split split_of(int dtype, long long M, int N, int K) {
   const long long t256 = (long long)((N + 255) / 256) * ((K + 255) / 256), t128 = (long long)((N + 127) / 128) * ((K + 127) / 128), stages = (M + 63) / 64;
-  if (t256 >= 192) return {256, 1, stages * 64};
+  if (t256 >= 192 && (dtype != SPB_F32 || N % 8 == 0)) return {256, 1, stages * 64};
   long long S = 256 / t128;
   if (S > stages / 4) S = stages / 4;
   if (S < 1) S = 1;
@@ -250,18 +253,25 @@ inline Split split_of(long long M, int N, int K) {
 }
 inline long long part_plane(int N, int K) { return (long long)N * ((K + 3) / 4 * 4); }
 
-template <typename T, int P, bool DMA, bool VEC, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
+template <typename T, int P, bool DMA, int MODE, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
   constexpr int LDS = 2 * (P + 1) * (P == 1 ? 64 : 32) * WN * TN * 16 * 2;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&wgrad8_kernel<T, P, DMA, VEC, WN, WK, TN, TK>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&wgrad8_kernel<T, P, DMA, MODE, WN, WK, TN, TK>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL((wgrad8_kernel<T, P, DMA, VEC, WN, WK, TN, TK>), dim3((unsigned)((long long)g.NT * g.KT * S)), dim3(WN * WK * 64), LDS, s, g);
+  hipLaunchKernelGGL((wgrad8_kernel<T, P, DMA, MODE, WN, WK, TN, TK>), dim3((unsigned)((long long)g.NT * g.KT * S)), dim3(WN * WK * 64), LDS, s, g);
   SPB_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, int P, bool DMA, bool VEC> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
+template <typename T, int P, bool DMA, int MODE> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
   g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
   if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
-  return sp.tile == 256 ? launch<T, P, DMA, VEC, 2, 4, 8, 4>(g, sp.S, s) : launch<T, P, DMA, VEC, 2, 2, 4, 4>(g, sp.S, s);
+  if constexpr (P < 3 || MODE == 0) {
+    if (sp.tile == 256) return launch<T, P, DMA, MODE, 2, 4, 8, 4>(g, sp.S, s);
+  }
+  return launch<T, P, DMA, MODE, 2, 2, 4, 4>(g, sp.S, s);
+}
+template <typename T, int P> int run_regs(const Wgrad8Args& g, const Split& sp, hipStream_t s) {
+  const int mode = vec_mode(g.N);
+  return mode == 0 ? run<T, P, false, 0>(g, sp, s) : (mode == 1 ? run<T, P, false, 1>(g, sp, s) : run<T, P, false, 2>(g, sp, s));
 }
 __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long ldw, int N, int K) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -274,7 +284,7 @@ __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long l
 extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
   if (M == 0 || N == 0 || K == 0) return 0;
-  const Split sp = split_of(M, N, K);
+  const Split sp = split_of(dtype, M, N, K);
   return sp.S > 1 ? (long long)sp.S * part_plane(N, K) * 4 : 0;
 }
 
@@ -292,20 +302,19 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
     return 0;
   }
   if (!a->G || !a->X || !a->Xs || ((uintptr_t)a->X & 15) || ((uintptr_t)a->Xs & 3)) return SPB_E_ARG;
-  const Split sp = split_of(a->M, a->N, a->K);
+  const Split sp = split_of(dtype, a->M, a->N, a->K);
   if (sp.S > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < spb_gemm8_wgrad_bytes(dtype, a->M, a->N, a->K))) return SPB_E_ARG;
-  const int es = dtype == SPB_F32 ? 4 : 2;
-  const bool vec = a->N % 8 == 0 && ((uintptr_t)a->G & 15) == 0 && (a->ldg * es) % 16 == 0;
   const long long plane = part_plane(a->N, a->K);
   const int outvec = ((uintptr_t)a->dW & 15) == 0 && a->ldw % 4 == 0;
   const Wgrad8Args g = {a->G, a->X, a->Xs, sp.S > 1 ? (float*)a->ws : a->dW, a->M, a->ldg, sp.S > 1 ? plane / a->N : a->ldw, sp.S > 1 ? plane : 0, sp.rows, a->N, a->K,
                         p8_cols(a->K), p8_scales(a->K), 0, 0, sp.S > 1 ? 0 : a->accumulate, sp.S > 1 ? 1 : outvec};
   int e;
-  if (dtype == SPB_F32) e = vec ? run<float, 3, false, true>(g, sp, s) : run<float, 3, false, false>(g, sp, s);
+  if (dtype == SPB_F32) e = run_regs<float, 3>(g, sp, s);
 #ifdef SPB_F16
-  else e = vec ? run<bf16_t, 2, false, true>(g, sp, s) : run<bf16_t, 2, false, false>(g, sp, s);
+  else e = run_regs<bf16_t, 2>(g, sp, s);
 #else
-  else e = vec && a->ldg < (1 << 24) ? run<bf16_t, 1, true, true>(g, sp, s) : run<bf16_t, 1, false, false>(g, sp, s);     // 64 rows: 32-bit offsets
+  else if (a->N % 8 == 0 && ((uintptr_t)a->G & 15) == 0 && a->ldg % 8 == 0 && a->ldg < (1 << 24)) e = run<bf16_t, 1, true, 0>(g, sp, s);   // 64 rows: 32-bit offsets
+  else e = run_regs<bf16_t, 1>(g, sp, s);
 #endif
   if (e) return e;
   if (sp.S > 1) {
