@@ -436,13 +436,7 @@ def layernorm_bwd(G, X, mean, rstd, gamma=None, dgamma=None, dbeta=None, dX=None
 class Packed8:
     """A matrix in e4m3 codes with one power-of-two scale for each block of 128 (include/spb_hip.h "8-bit packing"): codes uint8 [rows, K rounded up to
     128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight)."""
-    __slots__ = ("_codes", "_scales", "_K", "_block_rows", "_rows", "_dev")
-
-    codes = property(lambda self: self._codes)
-    scales = property(lambda self: self._scales)
-    K = property(lambda self: self._K)
-    block_rows = property(lambda self: self._block_rows)
-    shape = property(lambda self: (self._rows, self._K))
+    __slots__ = ("K", "block_rows", "shape", "_rows", "_dev", "_own", "_qp", "_sp")
 
     def __init__(self, codes, scales, K, block_rows):
         kb = (K + 127) // 128
@@ -452,28 +446,47 @@ class Packed8:
         for t, shape in ((codes, (rows, kb * 128)), (scales, ((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4))):
             if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
                 raise RuntimeError("Packed8: codes and scales do not fit a packed [%d, %d] matrix" % (rows, K))
-        self._set(codes, scales, K, block_rows, rows)
-
-    def _set(self, codes, scales, K, block_rows, rows):
-        self._codes, self._scales, self._K, self._block_rows, self._rows, self._dev = codes, scales, K, block_rows, rows, codes.get_device()
-        return self
+        self.K, self.block_rows, self.shape, self._rows, self._dev = K, block_rows, (rows, K), rows, codes.get_device()
+        self._own, self._qp, self._sp = (codes, scales), codes.data_ptr(), scales.data_ptr()
 
     @staticmethod
     def empty(rows, K, block_rows, device):
+        """uninitialised; codes and scales share one allocation"""
         kb = (K + 127) // 128
-        return Packed8.__new__(Packed8)._set(torch.empty((rows, kb * 128), dtype=torch.uint8, device=device),
-                                             torch.empty(((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4), dtype=torch.uint8, device=device),
-                                             K, block_rows, rows)
+        buf = torch.empty(rows * kb * 128 + (rows + block_rows - 1) // block_rows * ((kb + 3) // 4 * 4), dtype=torch.uint8, device=device)
+        self = Packed8.__new__(Packed8)
+        self.K, self.block_rows, self.shape, self._rows, self._dev = K, block_rows, (rows, K), rows, buf.get_device()
+        self._own, self._qp = buf, buf.data_ptr()
+        self._sp = self._qp + rows * kb * 128
+        return self
+
+    @property
+    def device(self):
+        return (self._own if isinstance(self._own, torch.Tensor) else self._own[0]).device
+
+    @property
+    def codes(self):
+        if isinstance(self._own, tuple):
+            return self._own[0]
+        kp = (self.K + 127) // 128 * 128
+        return self._own[:self._rows * kp].view(self._rows, kp)
+
+    @property
+    def scales(self):
+        if isinstance(self._own, tuple):
+            return self._own[1]
+        kb = (self.K + 127) // 128
+        return self._own[self._rows * kb * 128:].view((self._rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4)
 
 
 def _packed(P, name, dev=None, block_rows=None):
     """checks a Packed8 operand; returns its device"""
     if not isinstance(P, Packed8):
         raise RuntimeError("%s must be a Packed8 (quant8 / quant8_weight), got %s" % (name, type(P).__name__))
-    if block_rows is not None and P._block_rows != block_rows:
+    if block_rows is not None and P.block_rows != block_rows:
         raise RuntimeError("%s must be packed in blocks of %d x 128" % (name, block_rows))
     if P._dev < 0 or (dev is not None and P._dev != dev):
-        raise RuntimeError("%s is on %s, expected %s" % (name, P._codes.device, "a GPU" if dev is None else "device %d" % dev))
+        raise RuntimeError("%s is on %s, expected %s" % (name, P.device, "a GPU" if dev is None else "device %d" % dev))
     return P._dev
 
 
@@ -481,7 +494,7 @@ def quant8(X):
     """X [M, K] packed in blocks of 1 x 128: operand of gemm8 and checkpoint for gemm8_wgrad"""
     dev, M, K, ldx, code = _mat(X, "X")
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, P._codes.data_ptr(), P._scales.data_ptr())
+    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, P._qp, P._sp)
     return P
 
 
@@ -490,8 +503,8 @@ def quant8_weight(W, transpose=True):
     dev, N, K, ldw, code = _mat(W, "W")
     P = Packed8.empty(N, K, 128, W.device)
     T = Packed8.empty(K, N, 128, W.device) if transpose else None
-    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, P._codes.data_ptr(), P._scales.data_ptr(),
-          T._codes.data_ptr() if transpose else None, T._scales.data_ptr() if transpose else None)
+    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, P._qp, P._sp,
+          T._qp if transpose else None, T._sp if transpose else None)
     return P, T
 
 
@@ -499,9 +512,9 @@ def dequant8(P, dtype=torch.bfloat16, Y=None):
     """the values of a Packed8 (exact in bfloat16 and float32)"""
     dev = _packed(P, "P")
     if Y is None:
-        Y = torch.empty(P.shape, dtype=dtype, device=P._codes.device)
+        Y = torch.empty(P.shape, dtype=dtype, device=P.device)
     ldy = _out(Y, P.shape, dtype, "Y", dev)
-    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], P._codes.data_ptr(), P._scales.data_ptr(), P._block_rows, P._rows, P._K, Y.data_ptr(), ldy)
+    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], P._qp, P._sp, P.block_rows, P._rows, P.K, Y.data_ptr(), ldy)
     return Y
 
 
@@ -510,20 +523,20 @@ def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
     through the bfloat16 matrix instructions, where they are exact; 16-bit types: through the 8-bit ones."""
     dev = _packed(A, "A", None, 1)
     _packed(B, "B", dev)
-    if A._K != B._K:
-        raise RuntimeError("gemm8: A has %d columns, B has %d" % (A._K, B._K))
-    M, N, K = A._rows, B._rows, A._K
+    if A.K != B.K:
+        raise RuntimeError("gemm8: A has %d columns, B has %d" % (A.K, B.K))
+    M, N, K = A._rows, B._rows, A.K
     if dtype not in _DT:
         raise RuntimeError("gemm8 writes float32, bfloat16 or float16, not %s" % dtype)
     if Y is None:
-        Y, ldy = torch.empty((M, N), dtype=dtype, device=A._codes.device), N
+        Y, ldy = torch.empty((M, N), dtype=dtype, device=A.device), N
     else:
         ldy = _out(Y, (M, N), dtype, "Y", dev)
     lib, code = _lib8(dtype), _DT[dtype]
     need = lib.spb_gemm8_bytes(code, M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=A._codes.device) if need > 0 else None
-    a = A8.Gemm8Args(A._codes.data_ptr(), A._scales.data_ptr(), B._codes.data_ptr(), B._scales.data_ptr(), _vec(bias, N, "bias", dev), Y.data_ptr(),
-                     None if ws is None else ws.data_ptr(), need, M, ldy, N, K, B._block_rows)
+    ws = torch.empty(need, dtype=torch.uint8, device=A.device) if need > 0 else None
+    a = A8.Gemm8Args(A._qp, A._sp, B._qp, B._sp, _vec(bias, N, "bias", dev), Y.data_ptr(),
+                     None if ws is None else ws.data_ptr(), need, M, ldy, N, K, B.block_rows)
     _call(dev, lib.spb_gemm8, "spb_gemm8", code, C.byref(a))
     return Y
 
@@ -532,7 +545,7 @@ def gemm8_wgrad(G, X8, dW=None):
     """dW [N, K] (float32) = transpose of G [M, N] times the checkpoint X8 (quant8 of the layer's input [M, K]); dW given: accumulated into"""
     dev, M, N, ldg, code = _mat(G, "G")
     _packed(X8, "X8", dev, 1)
-    K = X8._K
+    K = X8.K
     if X8._rows != M:
         raise RuntimeError("gemm8_wgrad: G has %d rows, X8 has %d" % (M, X8._rows))
     accumulate = 0 if dW is None else 1
@@ -543,7 +556,7 @@ def gemm8_wgrad(G, X8, dW=None):
     lib = _lib8(G.dtype)
     need = lib.spb_gemm8_wgrad_bytes(code, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=G.device) if need > 0 else None
-    a = A8.Wgrad8Args(G.data_ptr(), X8._codes.data_ptr(), X8._scales.data_ptr(), dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
+    a = A8.Wgrad8Args(G.data_ptr(), X8._qp, X8._sp, dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
                       N, K, accumulate)
     _call(dev, lib.spb_gemm8_wgrad, "spb_gemm8_wgrad", code, C.byref(a))
     return dW
@@ -563,7 +576,7 @@ def act8_fwd(X, act, Y=None):
     else:
         ldy = _out(Y, (M, K), X.dtype, "Y", dev)
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, P._codes.data_ptr(), P._scales.data_ptr())
+    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, P._qp, P._sp)
     return Y, P
 
 
@@ -572,13 +585,13 @@ def act8_bwd(G, P, act, dX=None):
     _act8(act)
     dev, M, K, ldg, code = _mat(G, "G")
     _packed(P, "P", dev, 1)
-    if P._rows != M or P._K != K:
+    if P._rows != M or P.K != K:
         raise RuntimeError("act8_bwd: G is %s, the checkpoint %s" % ((M, K), P.shape))
     if dX is None:
         dX, ldd = G.new_empty((M, K)), K
     else:
         ldd = _out(dX, (M, K), G.dtype, "dX", dev)
-    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, P._codes.data_ptr(), P._scales.data_ptr(), dX.data_ptr(), ldd, M, K)
+    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, P._qp, P._sp, dX.data_ptr(), ldd, M, K)
     return dX
 
 
