@@ -5,8 +5,9 @@
 // the scale belongs to (m, 128 columns): along the reduction it changes with every step, which is why the 8-bit instructions, whose scale covers 32
 // steps of the reduction, do not fit.  G keeps all its bits: it is split by truncation into 1 (bfloat16), 2 (half: 8 + 3 bits) or 3 (float32: 8 + 8 + 8 bits)
 // bfloat16 pieces with an exact sum.
-//   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, or 128 x 128 with four of 64 x 64.  Stages of R rows (64; 32 with more than one piece) in LDS, two of
-//     them, read with the transpose load ds_read_b64_tr_b16.
+//   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; or 128 x 128, three stages ahead, with eight waves of 64 x 32 (one piece) or
+//     four of 64 x 64: a stage of the small tile is multiplied in a fifth of the time that memory takes to answer.  Stages of R rows (64; 32 with more than
+//     one piece) in LDS, read with the transpose load ds_read_b64_tr_b16.
 //   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
 //   * Few tiles and many rows: the rows are split over workgroups, each stores its partial tile, and a second launch adds them in order.
 // LDS rows hold TW columns without padding (the DMA image is linear).  The transpose load reads 32 bytes of 16 rows, r = 8 q + 0 .. 3 (+ 4): the 32-byte
@@ -25,38 +26,49 @@ struct Wgrad8Args {
   int N, K, Kp, Sp, NT, KT, accumulate, vec;           // vec: 16-byte stores fit the output
 };
 
-// bfloat16 pieces of 8 gradients: piece p of element i in out[p]
+// bfloat16 pieces of 8 gradients, piece p of all of them in out[p]: the upper half of the bits, then the same of what is left.  The differences are exact; a
+// gradient that is not finite leaves NaN in the second piece, and its row of dW is NaN.
 template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 out[P]) {
   float r[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = v[i];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    unsigned h[8];
+    unsigned u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned u = __float_as_uint(r[i]) & 0xffff0000u;
-      const bool fin = fabsf(r[i]) < __builtin_inff();
-      if (r[i] != r[i]) u = 0x7fc00000u;
-      h[i] = u;
-      r[i] = fin ? r[i] - __uint_as_float(u) : 0.f;     // exact: what the truncation cut off
-    }
-    out[p] = make_uint4((h[0] >> 16) | h[1], (h[2] >> 16) | h[3], (h[4] >> 16) | h[5], (h[6] >> 16) | h[7]);
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(r[i]);
+    out[p] = make_uint4(__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u),
+                        __builtin_amdgcn_perm(u[5], u[4], 0x07060302u), __builtin_amdgcn_perm(u[7], u[6], 0x07060302u));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(u[i] & 0xffff0000u);
   }
 }
 __device__ __forceinline__ int wg_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-// WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  DMA: G straight to LDS (P == 1, 16-byte aligned rows, MODE 0); otherwise through
-// registers (MODE: vec8.h)
-template <typename T, int P, bool DMA, int MODE, int WN, int WK, int TN, int TK>
+// WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  GDMA: G straight to LDS (P == 1, 16-byte aligned rows, MODE 0); otherwise through
+// registers (MODE: vec8.h).  Two forms:
+//   NST == 2 (large tile): X through registers requested a stage ahead; G by DMA (GDMA) or through registers too.
+//   NST > 2 (small tile): codes and scales of X come by DMA into a ring of NST stages and each lane turns what it fetched itself into bfloat16; G by DMA into
+//   a ring of its own or through registers.  (Several stages ahead in registers would not do for X: the compiler counts their loads without the DMA
+//   between them, and waits for all but the last stage.)
+template <typename T, int P, bool GDMA, int MODE, int NST, int WN, int WK, int TN, int TK>
 __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g) {
   constexpr int TW = WN * TN * 16, NW = WN * WK, NTH = NW * 64;
-  static_assert(WK * TK * 16 == TW && (!DMA || P == 1), "square tiles; DMA does not split");
-  constexpr int R = P == 1 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB, STAGE = (P + 1) * PLANE;
-  constexpr int DI = PLANE / 1024 / NW, RPI = 1024 / ROWB;              // DMA instructions of a stage for each wave, rows each covers
+  static_assert(WK * TK * 16 == TW, "square tiles");
+  constexpr bool RING = NST > 2;
+  static_assert(!GDMA || P == 1, "pieces come from registers");
+  constexpr int R = P == 1 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB;
   constexpr int XL = TW / 16, XR = NTH / XL, XP = R / XR;               // lanes of a row of codes (16 each), rows of a pass, passes
   constexpr int GL = TW / 8, GRW = NTH / GL, GP = R / GRW;              // the same for 8 gradients a lane
-  extern __shared__ __attribute__((aligned(16))) char smem[];           // two stages: P planes of G, one of X
+  constexpr int DI = GDMA ? PLANE / 1024 / NW : 0, RPI = 1024 / ROWB; // direct DMA: instructions of a stage for each wave, rows each covers
+  constexpr int IPS = DI + (RING ? 2 * XP : 0);
+  constexpr int GST = GDMA ? NST : 2 * P;                             // planes of G in LDS
+  constexpr int XOFF = GST * PLANE, XRAW = XOFF + 2 * PLANE, XST = NTH * XP * 20;
+  static_assert(XP * XR == R && GP * GRW == R && (!GDMA || DI * 1024 * NW == PLANE), "whole passes");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  // NST > 2: planes of G, two of X, the ring of X;  NST == 2: the planes of G and X of a stage side by side (their reads share address registers)
+  auto gplane = [&](int st, int slot) { return smem + (RING ? (GDMA ? slot * PLANE : (st & 1) * (P * PLANE)) : (st & 1) * ((P + 1) * PLANE)); };
+  auto xplane = [&](int st) { return smem + (RING ? XOFF + (st & 1) * PLANE : (st & 1) * ((P + 1) * PLANE) + P * PLANE); };
   const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wn = w / WK, wk = w % WK;
@@ -68,58 +80,75 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
 
   // ---- staging
   const unsigned lds0 = lds_addr(smem);
-  const int drow = w * RPI + l / (64 / RPI), dslot = l % (64 / RPI);                         // DMA: this lane's row of the first instruction, its 16-byte slot
+  const int drow = w * RPI + l / (64 / RPI), dslot = l % (64 / RPI);                         // direct DMA: this lane's row of the first instruction, its 16-byte slot
   int dcol = n0 + (((dslot >> 1) ^ wg_swz(drow)) * 2 + (dslot & 1)) * 8;                       // NW * RPI is a multiple of 16: the swizzle is the same in all
   dcol = dcol < g.N ? dcol : g.N - 8;                                                        // columns behind the matrix: any (not stored)
   const int xr = t / XL, xc = (t % XL) * 16;
   const int xk = k0 + xc < g.Kp ? k0 + xc : g.Kp - 16;
   const int gr = t / GL, gc = (t % GL) * 8;
-  uint4 xq[XP];
-  unsigned char xs[XP];
-  Raw8<T> graw[DMA ? 1 : GP];
-  auto fetch = [&](int st, int buf) {                    // requests stage st (its G by DMA into buffer `buf`)
+  struct Regs { uint4 xq[XP]; unsigned char xs[XP]; Raw8<T> graw[GDMA ? 1 : GP]; } regs;
+  auto rows_of = [&](int st) { const long long left = me - (mb + (long long)st * R); return (int)(left < R ? left : R); };
+  auto dma = [&](int st, int slot) {                     // what comes by DMA of stage st
     const long long m = mb + (long long)st * R;
-    const int last = (int)(me - 1 - m < R - 1 ? me - 1 - m : R - 1);
-    if constexpr (DMA) {
-      const char* base = reinterpret_cast<const char*>(g.G) + m * g.ldg * 2;
+    const int last = rows_of(st) - 1;
+    if constexpr (GDMA) {
+      const char* gb = reinterpret_cast<const char*>(g.G) + m * g.ldg * 2;
 #pragma unroll
       for (int i = 0; i < DI; ++i) {
         const int r = drow + i * (NW * RPI), rc = r < last ? r : last;
-        dma16s(base, ((unsigned)rc * (unsigned)g.ldg + (unsigned)dcol) * 2u, lds0 + (unsigned)(buf * STAGE + (i * NW + w) * 1024));
+        dma16s(gb, ((unsigned)rc * (unsigned)g.ldg + (unsigned)dcol) * 2u, lds0 + (unsigned)((RING ? slot * PLANE : (st & 1) * (2 * PLANE)) + (i * NW + w) * 1024));
       }
-    } else {
+    }
+    if constexpr (RING) {
+      const char* xb = reinterpret_cast<const char*>(g.X) + m * g.Kp;
+      const char* sb = reinterpret_cast<const char*>(g.Xs) + m * g.Sp;
+#pragma unroll
+      for (int i = 0; i < XP; ++i) {
+        const int r = xr + i * XR, rc = r < last ? r : last;
+        const unsigned to = lds0 + (unsigned)(XRAW + slot * XST);
+        dma16s(xb, (unsigned)rc * (unsigned)g.Kp + (unsigned)xk, to + (unsigned)((i * NW + w) * 1024));
+        dma4s(sb, (unsigned)rc * (unsigned)g.Sp + (unsigned)((xk >> 7) & ~3), to + (unsigned)(NTH * XP * 16 + (i * NW + w) * 256));
+      }
+    }
+  };
+  auto fetch = [&](int st) {                             // requests what goes through registers
+    const long long m = mb + (long long)st * R;
+    const int last = rows_of(st) - 1;
+    if constexpr (!GDMA) {
 #pragma unroll
       for (int i = 0; i < GP; ++i) {
-        const int r = gr + i * GRW, rc = r < last ? r : last;
+        const int r = gr + i * GRW, rc = r < last ? r : last, n = n0 + gc;
         const T* row = reinterpret_cast<const T*>(g.G) + (m + rc) * g.ldg;
-        const int n = n0 + gc;
         if constexpr (MODE == 2) {
           T e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = row[n + j < g.N ? n + j : 0];
-          __builtin_memcpy(&graw[i], e, sizeof(graw[i]));
+          __builtin_memcpy(&regs.graw[i], e, sizeof(regs.graw[i]));
         } else {
-          graw[i] = vec_get<T, MODE>(row, n, g.N);
+          regs.graw[i] = vec_get<T, MODE>(row, n, g.N);
         }
       }
     }
+    if constexpr (!RING) {
 #pragma unroll
-    for (int i = 0; i < XP; ++i) {
-      const int r = xr + i * XR, rc = r < last ? r : last;
-      xq[i] = *reinterpret_cast<const uint4*>(g.X + (m + rc) * g.Kp + xk);
-      xs[i] = g.Xs[(m + rc) * g.Sp + (xk >> 7)];
+      for (int i = 0; i < XP; ++i) {
+        const int r = xr + i * XR, rc = r < last ? r : last;
+        regs.xq[i] = *reinterpret_cast<const uint4*>(g.X + (m + rc) * g.Kp + xk);
+        regs.xs[i] = g.Xs[(m + rc) * g.Sp + (xk >> 7)];
+      }
     }
   };
-  auto commit = [&](int st, int buf) {                   // what came through registers goes to LDS; rows behind the last one as zeros
-    const long long left = me - (mb + (long long)st * R);
-    char* sb = smem + buf * STAGE;
-    if constexpr (!DMA) {
+  auto commit = [&](int st, int slot) {                  // stage st as bfloat16 into its planes; rows behind the last one as zeros
+    const int left = rows_of(st);
+    if constexpr (!GDMA) {
+      char* sb = gplane(st, slot);
 #pragma unroll
       for (int i = 0; i < GP; ++i) {
         const int r = gr + i * GRW;
+        Raw8<T> raw = regs.graw[i];
+        if constexpr (MODE == 1) vec_place<T, MODE>(raw, n0 + gc, g.N);
         float v[8];
-        if constexpr (MODE == 1) vec_place<T, MODE>(graw[i], n0 + gc, g.N);
-        cvt8(graw[i], v);
+        cvt8(raw, v);
         uint4 piece[P];
         split8<P>(v, piece);
 #pragma unroll
@@ -130,17 +159,30 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
 #pragma unroll
     for (int i = 0; i < XP; ++i) {
       const int r = xr + i * XR;
-      const float s = p8_pow2((int)xs[i] - 127);
-      const unsigned q[4] = {xq[i].x, xq[i].y, xq[i].z, xq[i].w};
+      uint4 xq;
+      unsigned xs;
+      if constexpr (RING) {
+        const char* q = smem + XRAW + slot * XST;
+        xq = *reinterpret_cast<const uint4*>(q + (i * NTH + t) * 16);
+        xs = *reinterpret_cast<const unsigned char*>(q + NTH * XP * 16 + (i * NTH + t) * 4 + ((xk >> 7) & 3));
+      } else {
+        xq = regs.xq[i];
+        xs = regs.xs[i];
+      }
+      const float s = p8_pow2((int)xs - 127);
+      const unsigned c[4] = {xq.x, xq.y, xq.z, xq.w};
       union { bf2_t h[8]; uint4 u[2]; } x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? q[j] : 0u, s, false);
-        x.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? q[j] : 0u, s, true);
+        x.h[2 * j] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? c[j] : 0u, s, false);
+        x.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? c[j] : 0u, s, true);
       }
-      char* p = sb + P * PLANE + r * ROWB + (((xc >> 4) ^ wg_swz(r)) << 5);
-      *reinterpret_cast<uint4*>(p) = x.u[0];
-      *reinterpret_cast<uint4*>(p + 16) = x.u[1];
+      // neighbouring lanes are 32 bytes apart: odd ones write their second half first, so that each instruction covers all banks
+      char* p = xplane(st) + r * ROWB + (((xc >> 4) ^ wg_swz(r)) << 5);
+      const bool odd = t & 1;
+      const uint4 u = x.u[0], v = x.u[1];                // (component by component: a choice between the two would put the array into scratch memory)
+      *reinterpret_cast<uint4*>(p + (odd ? 16 : 0)) = make_uint4(odd ? v.x : u.x, odd ? v.y : u.y, odd ? v.z : u.z, odd ? v.w : u.w);
+      *reinterpret_cast<uint4*>(p + (odd ? 0 : 16)) = make_uint4(odd ? u.x : v.x, odd ? u.y : v.y, odd ? u.z : v.z, odd ? u.w : v.w);
     }
   };
 
@@ -160,38 +202,101 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
     u.s.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4)(p + 4 * ROWB));
     return u.v;
   };
-  if (nst > 0) {
-    fetch(0, 0);
-    commit(0, 0);
-  }
-  wait_vmcnt<0>();
-  lds_barrier();
-  for (int st = 0; st < nst; ++st) {
-    const int buf = st & 1;
-    char* sb = smem + buf * STAGE;
-    if (DMA && me - (mb + (long long)st * R) < R) {       // the last stage is ragged: the rows that its DMA repeated are cleared
-      const int left = (int)(me - (mb + (long long)st * R));
-      for (int i = t + left * (ROWB / 16); i < R * (ROWB / 16); i += NTH) *reinterpret_cast<uint4*>(sb + i * 16) = make_uint4(0, 0, 0, 0);
+  auto clear = [&](int st, int slot) {                   // direct DMA repeats the last row of a ragged stage: those rows become zeros
+    if (GDMA && rows_of(st) < R) {
+      for (int i = t + rows_of(st) * (ROWB / 16); i < R * (ROWB / 16); i += NTH) *reinterpret_cast<uint4*>(gplane(st, slot) + i * 16) = make_uint4(0, 0, 0, 0);
       lds_barrier();
     }
-    if (st + 1 < nst) fetch(st + 1, buf ^ 1);
+  };
+  auto multiply = [&](int st, int slot) {
+    const char* sb = gplane(st, slot);
+    const char* sx = xplane(st);
+    if constexpr (RING) {                                 // every operand of the stage is read before the first product: one LDS round trip a stage
+      b16x8_t xf[R / 32][TK], gf[R / 32][P * TN];
 #pragma unroll
-    for (int mc = 0; mc < R / 32; ++mc) {
-      b16x8_t xf[TK];
+      for (int mc = 0; mc < R / 32; ++mc) {
 #pragma unroll
-      for (int b = 0; b < TK; ++b) xf[b] = trload(sb + P * PLANE, mc, wk * TK + b);
+        for (int b = 0; b < TK; ++b) xf[mc][b] = trload(sx, mc, wk * TK + b);
 #pragma unroll
-      for (int p = 0; p < P; ++p)
+        for (int pa = 0; pa < P * TN; ++pa) gf[mc][pa] = trload(sb + pa / TN * PLANE, mc, wn * TN + pa % TN);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int a = 0; a < TN; ++a) {
-          const b16x8_t gf = trload(sb + p * PLANE, mc, wn * TN + a);
+      for (int mc = 0; mc < R / 32; ++mc)
 #pragma unroll
-          for (int b = 0; b < TK; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[b], gf, acc[a][b], 0, 0, 0);
+        for (int pa = 0; pa < P * TN; ++pa)
+#pragma unroll
+          for (int b = 0; b < TK; ++b) acc[pa % TN][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[mc][b], gf[mc][pa], acc[pa % TN][b], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int mc = 0; mc < R / 32; ++mc) {
+        b16x8_t xf[TK], gf[2];
+        gf[0] = trload(sb, mc, wn * TN);
+#pragma unroll
+        for (int b = 0; b < TK; ++b) xf[b] = trload(sx, mc, wk * TK + b);
+#pragma unroll
+        for (int pa = 0; pa < P * TN; ++pa) {               // piece pa / TN, row tile pa % TN; the next one's operand is read under these products
+          if (pa + 1 < P * TN) gf[(pa + 1) & 1] = trload(sb + (pa + 1) / TN * PLANE, mc, wn * TN + (pa + 1) % TN);
+#pragma unroll
+          for (int b = 0; b < TK; ++b) acc[pa % TN][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[b], gf[pa & 1], acc[pa % TN][b], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
+      }
     }
-    if (st + 1 < nst) commit(st + 1, buf ^ 1);
+  };
+  if constexpr (RING) {
+    // NST - 1 stages are in flight.  While stage st is multiplied the buffer of stage st - 1 takes stage st + NST - 1; then this lane's part of stage st + 1
+    // has landed once only the stages behind it are in flight, and goes into its planes.
+    auto landed = [&](int st) {                          // stages behind st: at most NST - 2 have been requested
+      const int behind = nst - 1 - st;
+      if (behind >= NST - 2) wait_vmcnt<(NST - 2) * IPS>();
+      else if (behind == 1) wait_vmcnt<IPS>();
+      else wait_vmcnt<0>();
+    };
+    static_assert(NST == 4, "landed() knows 2, 1 or 0 stages behind");
+#pragma unroll
+    for (int q = 0; q < NST - 1; ++q)
+      if (q < nst) dma(q, q);
+    fetch(0);
+    landed(0);
+    commit(0, 0);
+    if (nst > 1) fetch(1);
+    lds_barrier();
+    int slot = 0;
+    for (int st = 0; st < nst; ++st) {
+      clear(st, slot);
+      if (st + NST - 1 < nst) dma(st + NST - 1, slot == 0 ? NST - 1 : slot - 1);
+      multiply(st, slot);
+      slot = slot == NST - 1 ? 0 : slot + 1;
+      if (st + 1 < nst) {
+        landed(st + 1);
+        commit(st + 1, slot);
+        if (st + 2 < nst) fetch(st + 2);
+      }
+      lds_barrier();
+    }
+  } else {
+    // While stage st is multiplied, stage st + 1 goes into the other buffers, its G by DMA, the rest from registers, which are then requested for stage
+    // st + 2.  In this order: the compiler waits for the registers' loads with a count that knows nothing of the DMA, so a DMA in front of the commit
+    // would be waited for there.
+    dma(0, 0);
+    fetch(0);
+    commit(0, 0);
+    if (nst > 1) fetch(1);
     wait_vmcnt<0>();
     lds_barrier();
+    for (int st = 0; st < nst; ++st) {
+      clear(st, st & 1);
+      if (st + 1 < nst) {
+        commit(st + 1, 0);
+        dma(st + 1, (st + 1) & 1);
+        if (st + 2 < nst) fetch(st + 2);
+      }
+      multiply(st, st & 1);
+      // the DMA has landed once only the requests of stage st + 2 (two for each pass over X) are in flight
+      if (GDMA) { if (st + 2 < nst) wait_vmcnt<2 * XP>(); else wait_vmcnt<0>(); }
+      lds_barrier();
+    }
   }
   // a lane holds four neighbouring k of one n
   float* out = g.out + (long long)split * g.plane;
@@ -253,21 +358,25 @@ inline Split split_of(int dtype, long long M, int N, int K) {
 }
 inline long long part_plane(int N, int K) { return (long long)N * ((K + 3) / 4 * 4); }
 
-template <typename T, int P, bool DMA, int MODE, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
-  constexpr int LDS = 2 * (P + 1) * (P == 1 ? 64 : 32) * WN * TN * 16 * 2;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&wgrad8_kernel<T, P, DMA, MODE, WN, WK, TN, TK>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+template <typename T, int P, bool GDMA, int MODE, int NST, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
+  constexpr int R = P == 1 ? 64 : 32, TW = WN * TN * 16, PLANE = R * TW * 2, NTH = WN * WK * 64;
+  constexpr int RING = NST > 2 ? NST * (R * TW + R * TW / 4) : 0;      // codes, a dword of scales a lane
+  constexpr int LDS = ((GDMA ? NST : 2 * P) + 2) * PLANE + RING;
+  static_assert(LDS <= 160 * 1024 && NTH * 16 <= R * TW, "fits a compute unit");
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&wgrad8_kernel<T, P, GDMA, MODE, NST, WN, WK, TN, TK>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return (int)e;
-  hipLaunchKernelGGL((wgrad8_kernel<T, P, DMA, MODE, WN, WK, TN, TK>), dim3((unsigned)((long long)g.NT * g.KT * S)), dim3(WN * WK * 64), LDS, s, g);
+  hipLaunchKernelGGL((wgrad8_kernel<T, P, GDMA, MODE, NST, WN, WK, TN, TK>), dim3((unsigned)((long long)g.NT * g.KT * S)), dim3(NTH), LDS, s, g);
   SPB_CHECK_LAUNCH();
   return 0;
 }
-template <typename T, int P, bool DMA, int MODE> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
+template <typename T, int P, bool GDMA, int MODE> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
   g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
   if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
   if constexpr (P < 3 || MODE == 0) {
-    if (sp.tile == 256) return launch<T, P, DMA, MODE, 2, 4, 8, 4>(g, sp.S, s);
+    if (sp.tile == 256) return launch<T, P, GDMA, MODE, 2, 2, 4, 8, 4>(g, sp.S, s);
   }
-  return launch<T, P, DMA, MODE, 2, 2, 4, 4>(g, sp.S, s);
+  if constexpr (P == 1) return launch<T, P, GDMA, MODE, 4, 2, 4, 4, 2>(g, sp.S, s);
+  else return launch<T, P, GDMA, MODE, 4, 2, 2, 4, 4>(g, sp.S, s);
 }
 template <typename T, int P> int run_regs(const Wgrad8Args& g, const Split& sp, hipStream_t s) {
   const int mode = vec_mode(g.N);
@@ -290,7 +399,7 @@ extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K)
 
 extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream_t stream) {
   if (!a || (dtype != SPB_F32 && dtype != SPB_BF16)) return SPB_E_ARG;
-  if (a->M < 0 || a->N < 0 || a->K < 0 || a->ldg < 0 || (a->N > 1 && a->ldw < a->K)) return SPB_E_SHAPE;
+  if (a->M < 0 || a->N < 0 || a->K < 0 || a->K > (1 << 23) || a->ldg < 0 || (a->N > 1 && a->ldw < a->K)) return SPB_E_SHAPE;     // 64 rows of codes: 32-bit offsets
   if (a->N == 0 || a->K == 0) return 0;
   if (!a->dW) return SPB_E_ARG;
   hipStream_t s = (hipStream_t)stream;
@@ -313,7 +422,8 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
 #ifdef SPB_F16
   else e = run_regs<bf16_t, 2>(g, sp, s);
 #else
-  else if (a->N % 8 == 0 && ((uintptr_t)a->G & 15) == 0 && a->ldg % 8 == 0 && a->ldg < (1 << 24)) e = run<bf16_t, 1, true, 0>(g, sp, s);   // 64 rows: 32-bit offsets
+  // by DMA: whole vectors at 16-byte addresses; the offsets of 64 rows fit 32 bits
+  else if (a->N % 8 == 0 && ((uintptr_t)a->G & 15) == 0 && a->ldg % 8 == 0 && a->ldg < (1 << 23)) e = run<bf16_t, 1, true, 0>(g, sp, s);
   else e = run_regs<bf16_t, 1>(g, sp, s);
 #endif
   if (e) return e;

@@ -95,7 +95,7 @@ def test_product_refusals(lib):
                 assert l.spb_gemm8(dt, product(M=M, N=N, K=K, ws=None), None) == ARG
     assert l.spb_gemm8_bytes(4, 1, 1, 1) < 0 and l.spb_gemm8_bytes(1, -1, 1, 1) < 0
     assert l.spb_gemm8_wgrad(2, wgrad(), None) == ARG and l.spb_gemm8_wgrad(1, None, None) == ARG
-    for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(ldg=-1), dict(ldw=255)):
+    for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(ldg=-1), dict(ldw=255), dict(K=(1 << 23) + 1)):
         assert l.spb_gemm8_wgrad(1, wgrad(**kw), None) == SHAPE, kw
     for kw in (dict(G=None), dict(X=None), dict(Xs=None), dict(dW=None), dict(X=ODD), dict(Xs=ODD), dict(ws=None), dict(ws=ODD),
                dict(ws_bytes=l.spb_gemm8_wgrad_bytes(1, 100000, 64, 256) - 1)):
