@@ -23,15 +23,9 @@ struct Gemm8Args {
   const float* bias; void* Y;
   long long M, ldy;
   long long plane;       // distance of two splits' outputs; 0: one split
-  int N, Kp, Sp, bshift, vec;
+  int N, Kp, Sp, bshift;
   int steps;             // steps of the reduction for each split
 };
-
-template <typename TO> __device__ __forceinline__ void store4(TO* p, const float v[4]);
-template <> __device__ __forceinline__ void store4<float>(float* p, const float v[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-template <> __device__ __forceinline__ void store4<bf16_t>(bf16_t* p, const float v[4]) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-}
 
 // 8 of a lane's 32 codes as bfloat16 values.  A and B give the same 8, so any order of the reduction will do.
 __device__ __forceinline__ b16x8_t wide8(const i32x8_t& f, int h, float s) {
@@ -52,22 +46,29 @@ __device__ __forceinline__ void dma4m(const void* sbase, unsigned voff, unsigned
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base) : "memory", "m0");
 }
 
-// bias, rounding and the store of four neighbouring columns of a row
-template <typename TO> __device__ __forceinline__ void put4(const Gemm8Args& g, TO* Y, long long m, int n, const f32x4_t& acc, const float bias[4]) {
-  float v[4];
+// bias, rounding and the store of V neighbouring columns of a row, at any alignment
+template <int V, typename TO> __device__ __forceinline__ void put(const Gemm8Args& g, TO* Y, long long m, int n, const f32x4_t* acc, const float bias[V]) {
+  float v[V];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) v[r] = acc[r] + bias[r];
+  for (int r = 0; r < V; ++r) v[r] = acc[r / 4][r % 4] + bias[r];
   TO* p = Y + m * g.ldy + n;
-  if (g.vec && n + 4 <= g.N) store4<TO>(p, v);
-  else {
+  if (n + V <= g.N) {
+    if constexpr (sizeof(TO) == 4) __builtin_memcpy(p, v, V * 4);
+    else {
+      unsigned u[V / 2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < V / 2; ++r) u[r] = pack_bf16x2(v[2 * r], v[2 * r + 1]);
+      __builtin_memcpy(p, u, V * 2);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < V; ++r)
       if (n + r < g.N) p[r] = from_f<TO>(v[r]);
   }
 }
-__device__ __forceinline__ void bias4(const Gemm8Args& g, int n, float bias[4]) {
+template <int V> __device__ __forceinline__ void bias_of(const Gemm8Args& g, int n, float bias[V]) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) bias[r] = g.bias != nullptr && n + r < g.N ? g.bias[n + r] : 0.f;
+  for (int r = 0; r < V; ++r) bias[r] = g.bias != nullptr && n + r < g.N ? g.bias[n + r] : 0.f;
 }
 
 constexpr int BAND = 8;      // tile rows that are walked together
@@ -79,6 +80,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   constexpr int DI = (BM + BN) / 8 / NW;                                // DMA instructions of a stage for each wave: 8 rows of codes each
   constexpr int ST = (BM + BN) / 64, SI = (ST + NW - 1) / NW;           // and 64 rows of scales each (a wave too many repeats an instruction)
   static_assert(DI * 8 * NW == BM + BN && ST * 64 == BM + BN, "whole DMA instructions");
+  // 16-bit output: the 16 rows of B in a pair of column tiles alternate in fours, so that a lane holds eight neighbouring columns and four lanes 64 bytes
+  constexpr bool PAIR = sizeof(TO) == 2;
+  static_assert(!PAIR || (TN % 2 == 0 && NW % 2 == 0), "pairs of column tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -98,13 +102,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   const char* abase = reinterpret_cast<const char*>(g.A) + m0 * g.Kp + (long long)kbeg * 128;
   const char* bbase = reinterpret_cast<const char*>(g.B) + (long long)n0 * g.Kp + (long long)kbeg * 128;
   const int mlast = (int)(g.M - 1 - m0 < BM - 1 ? g.M - 1 - m0 : BM - 1), nlast = g.N - 1 - n0 < BN - 1 ? g.N - 1 - n0 : BN - 1;
-  const int slot = ((l & 7) ^ (l >> 3)) << 4;
+  const int slot = ((l & 7) ^ (l >> 3)) << 4, slotb = PAIR ? ((l & 7) ^ ((l >> 3 & 3) | (w & 1) << 2)) << 4 : slot;
   unsigned off[DI], soff[SI];
 #pragma unroll
   for (int i = 0; i < DI; ++i) {
     const int r = (i * NW + w) * 8 + (l >> 3);
     const int rc = r < BM ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
-    off[i] = (unsigned)rc * (unsigned)g.Kp + (unsigned)slot;
+    off[i] = (unsigned)rc * (unsigned)g.Kp + (unsigned)((i * NW + w) * 8 < BM ? slot : slotb);
   }
   const char* asb = reinterpret_cast<const char*>(g.As) + m0 * g.Sp + kbeg;
   const char* bsb = reinterpret_cast<const char*>(g.Bs) + (long long)(n0 >> g.bshift) * g.Sp + kbeg;
@@ -152,8 +156,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
     else wait_vmcnt<0>();
     lds_barrier();
   };
-  const int ao = (wm * TM * 16 + li) * 128, bo = BM * 128 + (wn * TN * 16 + li) * 128;
-  const int ato = TILE + (wm * TM * 16 + li) * 4, bto = TILE + (BM + wn * TN * 16 + li) * 4;
+  const int ao = (wm * TM * 16 + li) * 128, bl = wn * TN * 16 + (PAIR ? (li >> 2) * 8 + (li & 3) : li), bo = BM * 128 + bl * 128;
+  const int ato = TILE + (wm * TM * 16 + li) * 4, bto = TILE + (BM + bl) * 4;
+  auto brow = [](int j) { return PAIR ? (j >> 1) * 32 + (j & 1) * 4 : j * 16; };      // row of column tile j behind this lane's first
   for (int s = 0; s < NST - 1 && s < KT; ++s) issue(s, s);
   int buf = 0;
   land(0);
@@ -161,7 +166,6 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
     // The operands of row tile i + 1 are read while row tile i is multiplied, and the next stage's DMA goes out between them: at the head of the step
     // its instructions would keep the first operand reads waiting.
     int sa[TM], sb[TN];
-    constexpr int AHEAD = 1;
     constexpr int PER = (DI + SI + TM - 1) / TM;
     for (int kt = 0; kt < KT; ++kt) {
       if (kt > 0) land(kt);
@@ -169,15 +173,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
       const int nbuf = buf == 0 ? NST - 1 : buf - 1;
       const bool more = kt + NST - 1 < KT;
       buf = buf == NST - 1 ? 0 : buf + 1;
-      i32x8_t b[TN], a[AHEAD + 1];
+      i32x8_t b[TN], a[2];
       a[0] = frag(stage + ao);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = frag(stage + bo + j * 2048);
-#pragma unroll
-      for (int i = 1; i < AHEAD && i < TM; ++i) a[i] = frag(stage + ao + i * 2048);
+      for (int j = 0; j < TN; ++j) b[j] = frag(stage + bo + brow(j) * 128);
       if ((kt & 3) == 0) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) sb[j] = *reinterpret_cast<const int*>(stage + bto + j * 64);
+        for (int j = 0; j < TN; ++j) sb[j] = *reinterpret_cast<const int*>(stage + bto + brow(j) * 4);
 #pragma unroll
         for (int i = 0; i < TM; ++i) sa[i] = *reinterpret_cast<const int*>(stage + ato + i * 64);
       } else {
@@ -188,9 +190,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
       }
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        if (i + AHEAD < TM) a[(i + AHEAD) % (AHEAD + 1)] = frag(stage + ao + (i + AHEAD) * 2048);
+        if (i + 1 < TM) a[(i + 1) & 1] = frag(stage + ao + (i + 1) * 2048);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i % (AHEAD + 1)], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
+        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
         if (more) {
 #pragma unroll
           for (int q = i * PER; q < (i + 1) * PER && q < DI + SI; ++q) issue1(q, kt + NST - 1, nbuf);
@@ -201,14 +203,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   } else {
     for (int kt = 0; kt < KT; ++kt) {
       if (kt > 0) land(kt);
-            if (kt + NST - 1 < KT) issue(kt + NST - 1, buf == 0 ? NST - 1 : buf - 1);
+      if (kt + NST - 1 < KT) issue(kt + NST - 1, buf == 0 ? NST - 1 : buf - 1);
       const char* stage = smem + buf * STAGE;
       buf = buf == NST - 1 ? 0 : buf + 1;
       i32x8_t b[TN], a[TM];
       float fa[TM], fb[TN];
       const int sh = (kt & 3) * 8;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) { b[j] = frag(stage + bo + j * 2048); fb[j] = scale_of(*reinterpret_cast<const unsigned*>(stage + bto + j * 64) >> sh); }
+      for (int j = 0; j < TN; ++j) { b[j] = frag(stage + bo + brow(j) * 128); fb[j] = scale_of(*reinterpret_cast<const unsigned*>(stage + bto + brow(j) * 4) >> sh); }
 #pragma unroll
       for (int i = 0; i < TM; ++i) { a[i] = frag(stage + ao + i * 2048); fa[i] = scale_of(*reinterpret_cast<const unsigned*>(stage + ato + i * 64) >> sh); }
 #pragma unroll
@@ -226,16 +228,17 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
     }
   }
 
+  constexpr int V = PAIR ? 8 : 4;
   TO* Y = reinterpret_cast<TO*>(g.Y) + split * g.plane;
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int n = n0 + (wn * TN + j) * 16 + lq * 4;
-    float bias[4];
-    bias4(g, n, bias);
+  for (int j = 0; j < TN; j += V / 4) {
+    const int n = n0 + wn * TN * 16 + j * 16 + lq * V;
+    float bias[V];
+    bias_of<V>(g, n, bias);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const long long m = m0 + (wm * TM + i) * 16 + li;
-      if (m < g.M) put4<TO>(g, Y, m, n, acc[i][j], bias);
+      if (m < g.M) put<V, TO>(g, Y, m, n, &acc[i][j], bias);
     }
   }
 }
@@ -294,8 +297,8 @@ __global__ __launch_bounds__(SKW * 64) void gemm8_rows_kernel(const Gemm8Args g)
     for (int k = 1; k < SKW; ++k) v += part[k][l];
     const int nn = n0 + lq * 4;
     float bias[4];
-    bias4(g, nn, bias);
-    if (li < g.M) put4<TO>(g, reinterpret_cast<TO*>(g.Y), li, nn, v, bias);
+    bias_of<4>(g, nn, bias);
+    if (li < g.M) put<4, TO>(g, reinterpret_cast<TO*>(g.Y), li, nn, &v, bias);
   }
 }
 
@@ -313,8 +316,8 @@ template <typename TO> __global__ __launch_bounds__(256) void gemm8_join_kernel(
     v += (f32x4_t){x.x, x.y, x.z, x.w};
   }
   float bias[4];
-  bias4(g, n, bias);
-  put4<TO>(g, reinterpret_cast<TO*>(g.Y), m, n, v, bias);
+  bias_of<4>(g, n, bias);
+  put<4, TO>(g, reinterpret_cast<TO*>(g.Y), m, n, &v, bias);
 }
 
 // no reduction (K == 0): the bias alone
@@ -366,7 +369,7 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
   if (c.tile >= 128) return run<128, 128, 2, EXACT ? 2 : 4, EXACT ? 2 : 4, EXACT, TO>(h, 1, s);
   if (c.S == 1) return run<64, 64, 2, 2, 4, EXACT, TO>(h, 1, s);
   const long long q = (g.N + 3) / 4, blocks = (g.M * q + 255) / 256;
-  h.Y = ws; h.bias = nullptr; h.ldy = 4 * q; h.plane = g.M * h.ldy; h.vec = 1;
+  h.Y = ws; h.bias = nullptr; h.ldy = 4 * q; h.plane = g.M * h.ldy;
   const int e = run<64, 64, 2, 2, 4, EXACT, float>(h, c.S, s);
   if (e) return e;
   Gemm8Args j = g;
@@ -390,10 +393,8 @@ extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stre
   if (a->M < 0 || a->N < 0 || a->K < 0 || a->K > (1 << 23) || (a->M > 1 && a->ldy < a->N)) return SPB_E_SHAPE;
   if (a->M == 0 || a->N == 0) return 0;
   if (!a->Y) return SPB_E_ARG;
-  const int es = dtype == SPB_F32 ? 4 : 2;
   hipStream_t s = (hipStream_t)stream;
-  Gemm8Args g = {a->A, a->As, a->B, a->Bs, a->bias, a->Y, a->M, a->ldy, 0, a->N, p8_cols(a->K), p8_scales(a->K), a->b_block_rows == 128 ? 7 : 0,
-                 ((uintptr_t)a->Y % (4 * es)) == 0 && a->ldy % 4 == 0, 0};
+  Gemm8Args g = {a->A, a->As, a->B, a->Bs, a->bias, a->Y, a->M, a->ldy, 0, a->N, p8_cols(a->K), p8_scales(a->K), a->b_block_rows == 128 ? 7 : 0, 0};
   if (a->K == 0) {
     const long long blocks = (a->M * a->N + 255) / 256;
     if (blocks > 0x7fffffffll) return SPB_E_SHAPE;
