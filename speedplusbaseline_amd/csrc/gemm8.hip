@@ -2,7 +2,7 @@
 //
 // The scales of a block of 128 are powers of two, the reduction step of v_mfma_scale_f32_16x16x128_f8f6f4 is 128 deep, and the instruction
 // multiplies by 2^(ea - 127) 2^(eb - 127) itself: a step of a tile is one instruction, and the sums of all blocks stay in one f32 accumulator.
-//   * Both operands go global -> LDS by LDS-DMA, 128 bytes of a row for each step, two stages.  The 16-byte slots of a row are XOR-swizzled with
+//   * Both operands go global -> LDS by LDS-DMA, 128 bytes of a row for each step, two or four stages.  The 16-byte slots of a row are XOR-swizzled with
 //     (row & 7) on the source address, so the lane-linear DMA image is read back without bank conflicts.
 //   * The scales of four steps are one dword a row: they ride the same DMA every fourth step.
 //   * The instruction's first operand is B: a lane then holds four neighbouring columns of one row of Y.
@@ -77,16 +77,19 @@ template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO>
 __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int TILE = (BM + BN) * 128, STAGE = TILE + (BM + BN) * 4;   // codes, then the dword of scales that holds this step's
-  constexpr int DI = (BM + BN) / 8 / NW;                                // DMA instructions of a stage for each wave: 8 rows of codes each
-  constexpr int ST = (BM + BN) / 64, SI = (ST + NW - 1) / NW;           // and 64 rows of scales each (a wave too many repeats an instruction)
-  static_assert(DI * 8 * NW == BM + BN && ST * 64 == BM + BN, "whole DMA instructions");
+  // Eight waves: the upper four, one on each SIMD, fetch at the head of a step, while the other four, whose instructions go first, multiply.  (All eight
+  // fetching between their products: 8192 x 8192 x 8192 419 us, like this 381; a wave that waits for a DMA instruction to be taken issues no product.)
+  constexpr bool LEAD = !EXACT && NW == 8;
+  constexpr int DW = LEAD ? NW / 2 : NW, DI = (BM + BN) / 8 / DW;       // waves that fetch; DMA instructions of a stage for each: 8 rows of codes
+  constexpr int ST = (BM + BN) / 64, SI = (ST + DW - 1) / DW;           // and 64 rows of scales each (a wave too many repeats an instruction)
+  static_assert(DI * 8 * DW == BM + BN && ST * 64 == BM + BN, "whole DMA instructions");
   // 16-bit output: the 16 rows of B in a pair of column tiles alternate in fours, so that a lane holds eight neighbouring columns and four lanes 64 bytes
   constexpr bool PAIR = sizeof(TO) == 2;
   static_assert(!PAIR || (TN % 2 == 0 && NW % 2 == 0), "pairs of column tiles");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int wm = w / WN, wn = w % WN;
+  const int wm = w / WN, wn = w % WN, wd = w % DW;
   // The 32 workgroups that an XCD runs at a time share one L2: eight tile rows times four tile columns of them fetch 12 tiles a step where a line of
   // 32 fetches 33 (8192 x 8192 x 8192: 4 TB/s out of the L2s' misses, half the matrix cores' time spent waiting).
   const int NT = (g.N + BN - 1) / BN, MT = (int)((g.M + BM - 1) / BM);
@@ -102,19 +105,19 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   const char* abase = reinterpret_cast<const char*>(g.A) + m0 * g.Kp + (long long)kbeg * 128;
   const char* bbase = reinterpret_cast<const char*>(g.B) + (long long)n0 * g.Kp + (long long)kbeg * 128;
   const int mlast = (int)(g.M - 1 - m0 < BM - 1 ? g.M - 1 - m0 : BM - 1), nlast = g.N - 1 - n0 < BN - 1 ? g.N - 1 - n0 : BN - 1;
-  const int slot = ((l & 7) ^ (l >> 3)) << 4, slotb = PAIR ? ((l & 7) ^ ((l >> 3 & 3) | (w & 1) << 2)) << 4 : slot;
+  const int slot = ((l & 7) ^ (l >> 3)) << 4, slotb = PAIR ? ((l & 7) ^ ((l >> 3 & 3) | (wd & 1) << 2)) << 4 : slot;
   unsigned off[DI], soff[SI];
 #pragma unroll
   for (int i = 0; i < DI; ++i) {
-    const int r = (i * NW + w) * 8 + (l >> 3);
+    const int r = (i * DW + wd) * 8 + (l >> 3);
     const int rc = r < BM ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
-    off[i] = (unsigned)rc * (unsigned)g.Kp + (unsigned)((i * NW + w) * 8 < BM ? slot : slotb);
+    off[i] = (unsigned)rc * (unsigned)g.Kp + (unsigned)((i * DW + wd) * 8 < BM ? slot : slotb);
   }
   const char* asb = reinterpret_cast<const char*>(g.As) + m0 * g.Sp + kbeg;
   const char* bsb = reinterpret_cast<const char*>(g.Bs) + (long long)(n0 >> g.bshift) * g.Sp + kbeg;
 #pragma unroll
   for (int i = 0; i < SI; ++i) {
-    const int r = (i * NW + w) % ST * 64 + l;
+    const int r = (i * DW + wd) % ST * 64 + l;
     const int rc = r < BM ? (r < mlast ? r : mlast) : (r - BM < nlast ? r - BM : nlast);
     soff[i] = (unsigned)(r < BM ? rc : ((n0 + rc) >> g.bshift) - (n0 >> g.bshift)) * (unsigned)g.Sp;
   }
@@ -122,14 +125,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   auto issue1 = [&](int i, int kt, int buf) {
     const unsigned sb = lds0 + (unsigned)(buf * STAGE);
     if (i < DI) {
-      const int r0 = (i * NW + w) * 8;
+      const int r0 = (i * DW + wd) * 8;
       dma16m((r0 < BM ? abase : bbase) + (size_t)kt * 128, off[i < DI ? i : 0], sb + (unsigned)(r0 * 128));
-    } else {
-      const int r0 = ((i - DI) * NW + w) % ST * 64;
+    } else if (EXACT || NST > 2 || (kt & 3) == 0) {        // (two stages, products: the dwords are read in the step they belong to only)
+      const int r0 = ((i - DI) * DW + wd) % ST * 64;
       dma4m((r0 < BM ? asb : bsb) + (kt & ~3), soff[i < DI ? 0 : i - DI], sb + (unsigned)(TILE + r0 * 4));
     }
   };
   auto issue = [&](int kt, int buf) {
+    if (LEAD && w >= DW) return;
 #pragma unroll
     for (int i = 0; i < DI + SI; ++i) issue1(i, kt, buf);
   };
@@ -163,9 +167,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   int buf = 0;
   land(0);
   if constexpr (!EXACT) {
-    // The operands of row tile i + 1 are read while row tile i is multiplied, and the next stage's DMA goes out between them: at the head of the step
-    // its instructions would keep the first operand reads waiting.
+    // The operands of row tile i + 1 are read while row tile i is multiplied.  Where every wave fetches, the next stage's DMA goes out between them: at the head of
+    // the step its instructions would keep the first operand reads waiting.
     int sa[TM], sb[TN];
+    if (LEAD && w >= DW) __builtin_amdgcn_s_setprio(1);
     constexpr int PER = (DI + SI + TM - 1) / TM;
     for (int kt = 0; kt < KT; ++kt) {
       if (kt > 0) land(kt);
@@ -174,6 +179,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
       const bool more = kt + NST - 1 < KT;
       buf = buf == NST - 1 ? 0 : buf + 1;
       i32x8_t b[TN], a[2];
+      if (LEAD && more) issue(kt + NST - 1, nbuf);
       a[0] = frag(stage + ao);
 #pragma unroll
       for (int j = 0; j < TN; ++j) b[j] = frag(stage + bo + brow(j) * 128);
@@ -193,7 +199,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
         if (i + 1 < TM) a[(i + 1) & 1] = frag(stage + ao + (i + 1) * 2048);
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i & 1], acc[i][j], 0, 0, 0, sb[j], 0, sa[i]);
-        if (more) {
+        if (!LEAD && more) {
 #pragma unroll
           for (int q = i * PER; q < (i + 1) * PER && q < DI + SI; ++q) issue1(q, kt + NST - 1, nbuf);
         }
@@ -340,14 +346,15 @@ template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int 
 }
 
 constexpr long long ROWS_MAX = 16;
-// How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 282 us, 128 x 128: 301 us) but leave compute units idle below about 192 of
-// them (2352 x 1024 x 1280: 24 against 11 us); 128 x 128 tiles are used down to 128 of those.  Smaller products take 64 x 64 tiles, and where even these are
-// fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up.
+// How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 211 us, 128 x 128: 261 us) but leave compute units idle below about 144 of
+// them (2816 x 4096 x 4096, 176 tiles: 49 against 54 us; 2048 x 4096 x 2048, 128 tiles: 28 against 22 us).  128 x 128 tiles are used down to as many
+// (2352 x 1024 x 1024, 152 tiles: 8.4 us, 64 x 64: 10.1; 2048 x 1024 x 1024, 128 tiles: 8.3 and 7.0).  Smaller products take 64 x 64 tiles, and where
+// even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up.
 struct Cut { int tile, S, steps; };
 inline Cut cut_of(long long M, int N, int KT) {
   const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
-  if (t256 >= 192) return {256, 1, (KT + 3) / 4 * 4};
-  if (t128 >= 128) return {128, 1, (KT + 3) / 4 * 4};
+  if (t256 >= 144) return {256, 1, (KT + 3) / 4 * 4};
+  if (t128 >= 144) return {128, 1, (KT + 3) / 4 * 4};
   long long S = t64 >= 256 ? 1 : 256 / t64;
   const int quads = (KT + 3) / 4;
   if (S > quads) S = quads;
@@ -366,7 +373,12 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
   if constexpr (!EXACT) {
     if (c.tile == 256) return run<256, 256, 2, 4, 2, false, TO>(h, 1, s);
   }
-  if (c.tile >= 128) return run<128, 128, 2, EXACT ? 2 : 4, EXACT ? 2 : 4, EXACT, TO>(h, 1, s);
+  if (c.tile >= 128) {
+    // more tiles than compute units: two workgroups on each cover each other's waits (3840 x 2048 x 2048: 25.6 -> 22.1 us); fewer: four stages do (4096 x 1024 x 4096: 26.7 -> 24.4)
+    if constexpr (EXACT) return run<128, 128, 2, 2, 2, true, TO>(h, 1, s);
+    else if ((g.M + 127) / 128 * ((g.N + 127) / 128) > 256) return run<128, 128, 2, 4, 2, false, TO>(h, 1, s);
+    else return run<128, 128, 2, 4, 4, false, TO>(h, 1, s);
+  }
   if (c.S == 1) return run<64, 64, 2, 2, 4, EXACT, TO>(h, 1, s);
   const long long q = (g.N + 3) / 4, blocks = (g.M * q + 255) / 256;
   h.Y = ws; h.bias = nullptr; h.ldy = 4 * q; h.plane = g.M * h.ldy;
