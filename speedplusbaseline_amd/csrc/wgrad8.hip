@@ -8,7 +8,10 @@
 //   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; or 128 x 128, three stages ahead, with eight waves of 64 x 32 (one piece) or
 //     four of 64 x 64: a stage of the small tile is multiplied in a fifth of the time that memory takes to answer.  Stages of R rows (64; 32 with more than
 //     one piece) in LDS, read with the transpose load ds_read_b64_tr_b16.
+//     The large tile is bound by LDS as much as by the products: 64 rows are 2048 clocks of matrix instructions, and 1536 of reads and 512 of writes in LDS.
 //   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
+//   * Of the two waves on a SIMD one multiplies a stage before it brings the next one into place, the other after it: the matrix cores work while operands are
+//     converted (16384 x 4096 x 4096: 459 -> 427 us; 37632 x 1024 x 1280: 183 -> 174).
 //   * Few tiles and many rows: the rows are split over workgroups, each stores its partial tile, and a second launch adds them in order.
 // LDS rows hold TW columns without padding (the DMA image is linear).  The transpose load reads 32 bytes of 16 rows, r = 8 q + 0 .. 3 (+ 4): the 32-byte
 // pairs of a row are XOR-swizzled with (r & 3) + 4 ((r >> 3) & 1), which spreads them over all banks.
@@ -60,11 +63,12 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   constexpr int R = P == 1 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB;
   constexpr int XL = TW / 16, XR = NTH / XL, XP = R / XR;               // lanes of a row of codes (16 each), rows of a pass, passes
   constexpr int GL = TW / 8, GRW = NTH / GL, GP = R / GRW;              // the same for 8 gradients a lane
-  constexpr int DI = GDMA ? PLANE / 1024 / NW : 0, RPI = 1024 / ROWB; // direct DMA: instructions of a stage for each wave, rows each covers
+  constexpr int DW = RING ? NW : NW / 2, DI = GDMA ? PLANE / 1024 / DW : 0, RPI = 1024 / ROWB; // direct DMA: waves that issue it (large tile: those that multiply
+                                                                        // last), instructions of a stage for each, rows each covers
   constexpr int IPS = DI + (RING ? 2 * XP : 0);
   constexpr int GST = GDMA ? NST : 2 * P;                             // planes of G in LDS
   constexpr int XOFF = GST * PLANE, XRAW = XOFF + 2 * PLANE, XST = NTH * XP * 20;
-  static_assert(XP * XR == R && GP * GRW == R && (!GDMA || DI * 1024 * NW == PLANE), "whole passes");
+  static_assert(XP * XR == R && GP * GRW == R && (!GDMA || DI * 1024 * DW == PLANE), "whole passes");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   // NST > 2: planes of G, two of X, the ring of X;  NST == 2: the planes of G and X of a stage side by side (their reads share address registers)
   auto gplane = [&](int st, int slot) { return smem + (RING ? (GDMA ? slot * PLANE : (st & 1) * (P * PLANE)) : (st & 1) * ((P + 1) * PLANE)); };
@@ -72,6 +76,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   const int t = threadIdx.x, l = t & 63, li = l & 15, lq = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wn = w / WK, wk = w % WK;
+  const bool first = w >= NW / 2;                        // this wave multiplies first
   const int lid = xcd_remap(blockIdx.x, gridDim.x);     // the tiles of a split read the same rows: one XCD, back to back
   const int tiles = g.NT * g.KT, tile = lid % tiles, split = lid / tiles;
   const int n0 = (tile / g.KT) * TW, k0 = (tile % g.KT) * TW;
@@ -81,8 +86,12 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   // ---- staging
   const unsigned lds0 = lds_addr(smem);
   const int drow = w * RPI + l / (64 / RPI), dslot = l % (64 / RPI);                         // direct DMA: this lane's row of the first instruction, its 16-byte slot
-  int dcol = n0 + (((dslot >> 1) ^ wg_swz(drow)) * 2 + (dslot & 1)) * 8;                       // NW * RPI is a multiple of 16: the swizzle is the same in all
-  dcol = dcol < g.N ? dcol : g.N - 8;                                                        // columns behind the matrix: any (not stored)
+  int dcol[2];                                             // every other pass has the other half of the swizzle where a pass covers 8 rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = n0 + (((dslot >> 1) ^ wg_swz(drow + i * DW * RPI)) * 2 + (dslot & 1)) * 8;
+    dcol[i] = c < g.N ? c : g.N - 8;                       // columns behind the matrix: any (not stored)
+  }
   const int xr = t / XL, xc = (t % XL) * 16;
   const int xk = k0 + xc < g.Kp ? k0 + xc : g.Kp - 16;
   const int gr = t / GL, gc = (t % GL) * 8;
@@ -95,8 +104,8 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
       const char* gb = reinterpret_cast<const char*>(g.G) + m * g.ldg * 2;
 #pragma unroll
       for (int i = 0; i < DI; ++i) {
-        const int r = drow + i * (NW * RPI), rc = r < last ? r : last;
-        dma16s(gb, ((unsigned)rc * (unsigned)g.ldg + (unsigned)dcol) * 2u, lds0 + (unsigned)((RING ? slot * PLANE : (st & 1) * (2 * PLANE)) + (i * NW + w) * 1024));
+        const int r = drow + i * (DW * RPI), rc = r < last ? r : last;
+        dma16s(gb, ((unsigned)rc * (unsigned)g.ldg + (unsigned)dcol[i & 1]) * 2u, lds0 + (unsigned)((RING ? slot * PLANE : (st & 1) * (2 * PLANE)) + (i * DW + w) * 1024));
       }
     }
     if constexpr (RING) {
@@ -245,8 +254,8 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
     }
   };
   if constexpr (RING) {
-    // NST - 1 stages are in flight.  While stage st is multiplied the buffer of stage st - 1 takes stage st + NST - 1; then this lane's part of stage st + 1
-    // has landed once only the stages behind it are in flight, and goes into its planes.
+    // NST - 1 stages are in flight.  Before or after stage st is multiplied the buffer of stage st - 1 takes stage st + NST - 1, and this lane's part of stage st + 1, which
+    // has landed once only the stages behind it are in flight, goes into its planes.
     auto landed = [&](int st) {                          // stages behind st: at most NST - 2 have been requested
       const int behind = nst - 1 - st;
       if (behind >= NST - 2) wait_vmcnt<(NST - 2) * IPS>();
@@ -265,21 +274,23 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
     int slot = 0;
     for (int st = 0; st < nst; ++st) {
       clear(st, slot);
+      const int next = slot == NST - 1 ? 0 : slot + 1;
+      if (first) multiply(st, slot);
       if (st + NST - 1 < nst) dma(st + NST - 1, slot == 0 ? NST - 1 : slot - 1);
-      multiply(st, slot);
-      slot = slot == NST - 1 ? 0 : slot + 1;
       if (st + 1 < nst) {
         landed(st + 1);
-        commit(st + 1, slot);
+        commit(st + 1, next);
         if (st + 2 < nst) fetch(st + 2);
       }
+      if (!first) multiply(st, slot);
+      slot = next;
       lds_barrier();
     }
   } else {
-    // While stage st is multiplied, stage st + 1 goes into the other buffers, its G by DMA, the rest from registers, which are then requested for stage
-    // st + 2.  In this order: the compiler waits for the registers' loads with a count that knows nothing of the DMA, so a DMA in front of the commit
+    // Before or after stage st is multiplied, stage st + 1 goes into the other buffers, its G by DMA, the rest from registers, which are then requested for
+    // stage st + 2.  In this order: the compiler waits for the registers' loads with a count that knows nothing of the DMA, so a DMA in front of the commit
     // would be waited for there.
-    dma(0, 0);
+    if (!first) dma(0, 0);
     fetch(0);
     commit(0, 0);
     if (nst > 1) fetch(1);
@@ -287,14 +298,17 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
     lds_barrier();
     for (int st = 0; st < nst; ++st) {
       clear(st, st & 1);
+      if (first) multiply(st, st & 1);
       if (st + 1 < nst) {
         commit(st + 1, 0);
-        dma(st + 1, (st + 1) & 1);
+        if (!first) dma(st + 1, (st + 1) & 1);
         if (st + 2 < nst) fetch(st + 2);
       }
-      multiply(st, st & 1);
-      // the DMA has landed once only the requests of stage st + 2 (two for each pass over X) are in flight
-      if (GDMA) { if (st + 2 < nst) wait_vmcnt<2 * XP>(); else wait_vmcnt<0>(); }
+      if (!first) {
+        multiply(st, st & 1);
+        // the DMA has landed once only the requests of stage st + 2 (two for each pass over X) are in flight
+        if (GDMA) { if (st + 2 < nst) wait_vmcnt<2 * XP>(); else wait_vmcnt<0>(); }
+      }
       lds_barrier();
     }
   }
