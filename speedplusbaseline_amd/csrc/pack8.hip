@@ -16,21 +16,25 @@ __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, spb_dpp_f<0xB1>(v)); v = fmaxf(v, spb_dpp_f<0x4E>(v)); v = fmaxf(v, spb_dpp_f<0x141>(v)); v = fmaxf(v, spb_dpp_f<0x140>(v));
   return v;
 }
-// 8 elements from column c on, zeros behind K (MODE: vec8.h)
-template <typename T, int MODE> __device__ __forceinline__ void load8(const T* row, int c, int K, float v[8]) {
+// 8 elements from column c on (MODE: vec8.h): requested, then put into place with zeros behind K
+template <typename T, int MODE> __device__ __forceinline__ Raw8<T> get8(const T* row, int c, int K) {
   if constexpr (MODE == 2) {
     T t[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = row[c + i < K ? c + i : 0];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < K ? to_f<T>(t[i]) : 0.f;
+    return vec_ld<T>(t);
   } else {
-    Raw8<T> r = vec_get<T, MODE>(row, c, K);
-    vec_place<T, MODE>(r, c, K);
-    cvt8(r, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + (MODE == 0 ? 0 : i) < K ? v[i] : 0.f;
+    return vec_get<T, MODE>(row, c, K);
   }
+}
+template <typename T, int MODE> __device__ __forceinline__ void place8(Raw8<T> r, int c, int K, float v[8]) {
+  vec_place<T, MODE>(r, c, K);
+  cvt8(r, v);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = c + (MODE == 0 ? 0 : i) < K ? v[i] : 0.f;
+}
+template <typename T, int MODE> __device__ __forceinline__ void load8(const T* row, int c, int K, float v[8]) {
+  place8<T, MODE>(get8<T, MODE>(row, c, K), c, K, v);
 }
 // The f32 value is what is rounded, in both forms: without the empty asm the compiler may fold a product into its conversion to half (one rounding
 // instead of two) in one of them, and a result would depend on its row's length.
@@ -148,10 +152,17 @@ __global__ __launch_bounds__(256) void pack8_weight_kernel(const WeightArgs a) {
   const int nb = blockIdx.x / a.KB, kb = blockIdx.x - nb * a.KB;
   const int l = threadIdx.x & 15, r0 = (threadIdx.x >> 4) * 8, c = kb * P8_BLOCK + l * 8;
   float v[8][8];
+  Raw8<T> raw[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int n = nb * P8_BLOCK + r0 + i;
-    load8<T, MODE>(reinterpret_cast<const T*>(a.W) + (long long)(n < a.N ? n : 0) * a.ldw, c, a.K, v[i]);
+    raw[i] = get8<T, MODE>(reinterpret_cast<const T*>(a.W) + (long long)(n < a.N ? n : 0) * a.ldw, c, a.K);
+  }
+  __builtin_amdgcn_sched_barrier(0);                   // all requests before the first is used (4096 x 4096 f32: 17.4 -> 16.9 us)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int n = nb * P8_BLOCK + r0 + i;
+    place8<T, MODE>(raw[i], c, a.K, v[i]);
     if (n >= a.N) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;

@@ -22,12 +22,17 @@ __device__ __forceinline__ void vec_shift(Raw8<bf16_t>& r, int s) {
   r.u = make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
 }
 __device__ __forceinline__ void vec_shift(Raw8<float>& r, int s) {
-  float v[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  // bit masks: of `s & k ? v[i + k] : v[i]` the compiler makes eight comparisons for each element
+  unsigned v[8] = {__float_as_uint(r.a.x), __float_as_uint(r.a.y), __float_as_uint(r.a.z), __float_as_uint(r.a.w),
+                   __float_as_uint(r.b.x), __float_as_uint(r.b.y), __float_as_uint(r.b.z), __float_as_uint(r.b.w)};
 #pragma unroll
-  for (int k = 1; k < 8; k <<= 1)
+  for (int k = 1; k < 8; k <<= 1) {
+    const unsigned m = s & k ? 0xffffffffu : 0u;
 #pragma unroll
-    for (int i = 0; i + k < 8; ++i) v[i] = s & k ? v[i + k] : v[i];
-  r.a = make_float4(v[0], v[1], v[2], v[3]); r.b = make_float4(v[4], v[5], v[6], v[7]);
+    for (int i = 0; i + k < 8; ++i) v[i] = (v[i + k] & m) | (v[i] & ~m);
+  }
+  r.a = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+  r.b = make_float4(__uint_as_float(v[4]), __uint_as_float(v[5]), __uint_as_float(v[6]), __uint_as_float(v[7]));
 }
 // where the vector of column c is loaded from (c >= C: anywhere in the row; its elements are not used)
 template <int MODE> __device__ __forceinline__ int vec_from(int c, int C) { return MODE == 0 ? (c < C ? c : 0) : (c + 8 <= C ? c : C - 8); }

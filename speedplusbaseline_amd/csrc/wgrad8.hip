@@ -360,10 +360,9 @@ __global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int
 struct Split { int tile, S; long long rows; };
 // 256 x 256 tiles where at least 192 of them keep the compute units busy, otherwise 128 x 128 with the rows split for at least 256 workgroups, four
 // stages in each
-// (f32 gradients with rows that end inside a vector: three pieces and the shift into place do not fit the registers of the large tile)
-inline Split split_of(int dtype, long long M, int N, int K) {
+inline Split split_of(long long M, int N, int K) {
   const long long t256 = (long long)((N + 255) / 256) * ((K + 255) / 256), t128 = (long long)((N + 127) / 128) * ((K + 127) / 128), stages = (M + 63) / 64;
-  if (t256 >= 192 && (dtype != SPB_F32 || N % 8 == 0)) return {256, 1, stages * 64};
+  if (t256 >= 192) return {256, 1, stages * 64};
   long long S = 256 / t128;
   if (S > stages / 4) S = stages / 4;
   if (S < 1) S = 1;
@@ -386,9 +385,7 @@ template <typename T, int P, bool GDMA, int MODE, int NST, int WN, int WK, int T
 template <typename T, int P, bool GDMA, int MODE> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
   g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
   if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
-  if constexpr (P < 3 || MODE == 0) {
-    if (sp.tile == 256) return launch<T, P, GDMA, MODE, 2, 2, 4, 8, 4>(g, sp.S, s);
-  }
+  if (sp.tile == 256) return launch<T, P, GDMA, MODE, 2, 2, 4, 8, 4>(g, sp.S, s);
   if constexpr (P == 1) return launch<T, P, GDMA, MODE, 4, 2, 4, 4, 2>(g, sp.S, s);
   else return launch<T, P, GDMA, MODE, 4, 2, 2, 4, 4>(g, sp.S, s);
 }
@@ -407,7 +404,7 @@ __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long l
 extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
   if (M == 0 || N == 0 || K == 0) return 0;
-  const Split sp = split_of(dtype, M, N, K);
+  const Split sp = split_of(M, N, K);
   return sp.S > 1 ? (long long)sp.S * part_plane(N, K) * 4 : 0;
 }
 
@@ -425,7 +422,7 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
     return 0;
   }
   if (!a->G || !a->X || !a->Xs || ((uintptr_t)a->X & 15) || ((uintptr_t)a->Xs & 3)) return SPB_E_ARG;
-  const Split sp = split_of(dtype, a->M, a->N, a->K);
+  const Split sp = split_of(a->M, a->N, a->K);
   if (sp.S > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < spb_gemm8_wgrad_bytes(dtype, a->M, a->N, a->K))) return SPB_E_ARG;
   const long long plane = part_plane(a->N, a->K);
   const int outvec = ((uintptr_t)a->dW & 15) == 0 && a->ldw % 4 == 0;
