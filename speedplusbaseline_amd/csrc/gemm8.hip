@@ -308,19 +308,15 @@ __global__ __launch_bounds__(SKW * 64) void gemm8_rows_kernel(const Gemm8Args g)
   }
 }
 
-// Y = the S partial products, in order, + bias: four columns a thread
-template <typename TO> __global__ __launch_bounds__(256) void gemm8_join_kernel(const Gemm8Args g, const float* part, int S) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+// Y = the S partial products + bias: four columns a thread, partial rows hold a multiple of four
+template <typename TO, int GR> __global__ __launch_bounds__(256) void gemm8_join_kernel(const Gemm8Args g, const float* part, int S) {
+  long long i;
+  float4 x;
+  if (!p8_sum_parts<GR>(part, S, g.plane, i, x)) return;
   const int q = (g.N + 3) >> 2;
   const long long m = i / q;
   const int n = (int)(i - m * q) * 4;
-  if (m >= g.M) return;
-  f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < S; ++s) {
-    const float* p = part + s * g.plane + m * (4 * q) + n;        // partial rows hold a multiple of four columns
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v += (f32x4_t){x.x, x.y, x.z, x.w};
-  }
+  const f32x4_t v = {x.x, x.y, x.z, x.w};
   float bias[4];
   bias_of<4>(g, n, bias);
   put<4, TO>(g, reinterpret_cast<TO*>(g.Y), m, n, &v, bias);
@@ -380,13 +376,15 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
     else return run<128, 128, 2, 4, 4, false, TO>(h, 1, s);
   }
   if (c.S == 1) return run<64, 64, 2, 2, 4, EXACT, TO>(h, 1, s);
-  const long long q = (g.N + 3) / 4, blocks = (g.M * q + 255) / 256;
+  const long long q = (g.N + 3) / 4;
   h.Y = ws; h.bias = nullptr; h.ldy = 4 * q; h.plane = g.M * h.ldy;
   const int e = run<64, 64, 2, 2, 4, EXACT, float>(h, c.S, s);
   if (e) return e;
   Gemm8Args j = g;
   j.plane = h.plane;
-  hipLaunchKernelGGL((gemm8_join_kernel<TO>), dim3((unsigned)blocks), dim3(256), 0, s, j, (const float*)ws, c.S);
+  const dim3 blocks((unsigned)p8_join_blocks(h.plane, c.S));
+  if (c.S > P8_JOIN) hipLaunchKernelGGL((gemm8_join_kernel<TO, 16>), blocks, dim3(256), 0, s, j, (const float*)ws, c.S);
+  else hipLaunchKernelGGL((gemm8_join_kernel<TO, 1>), blocks, dim3(256), 0, s, j, (const float*)ws, c.S);
   SPB_CHECK_LAUNCH();
   return 0;
 }

@@ -53,3 +53,34 @@ __device__ __forceinline__ void dma4s(const void* sbase, unsigned voff, unsigned
   asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(keep) : "v"(voff), "s"(sbase), "s"(lds_base) : "memory");
 }
+
+// Sum of S partial planes in a fixed order, four neighbouring floats a thread (`i` is their number).  GR 1: a thread adds all of them, four requested at a time.
+// Many planes (S > P8_JOIN): GR threads take a part of the planes each, whose sums meet in LDS; one of them returns true with the result.
+constexpr int P8_JOIN = 16;
+template <int GR> __device__ __forceinline__ bool p8_sum_parts(const float* part, int S, long long plane, long long& i, float4& v) {
+  constexpr int Q = 256 / GR;
+  const int ql = threadIdx.x % Q, gr = threadIdx.x / Q, per = (S + GR - 1) / GR, s0 = gr * per, s1 = s0 + per < S ? s0 + per : S;
+  i = (long long)blockIdx.x * Q + ql;
+  const bool in = i * 4 < plane;
+  const float* p = part + (in ? i * 4 : 0);
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int B = GR == 1 ? 4 : 8;
+  for (int s = s0; s < s1; s += B) {
+    float4 x[B];
+#pragma unroll
+    for (int k = 0; k < B; ++k) x[k] = *reinterpret_cast<const float4*>(p + (s + k < s1 ? s + k : s1 - 1) * plane);
+#pragma unroll
+    for (int k = 0; k < B; ++k)
+      if (s + k < s1) { v.x += x[k].x; v.y += x[k].y; v.z += x[k].z; v.w += x[k].w; }
+  }
+  if constexpr (GR > 1) {
+    __shared__ float4 red[GR][Q];
+    red[gr][ql] = v;
+    __syncthreads();
+    if (gr > 0) return false;
+#pragma unroll
+    for (int k = 1; k < GR; ++k) { const float4 x = red[k][ql]; v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w; }
+  }
+  return in;
+}
+inline long long p8_join_blocks(long long plane, int S) { const int q = S > P8_JOIN ? 16 : 256; return (plane / 4 + q - 1) / q; }

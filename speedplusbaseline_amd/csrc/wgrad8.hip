@@ -5,16 +5,17 @@
 // the scale belongs to (m, 128 columns): along the reduction it changes with every step, which is why the 8-bit instructions, whose scale covers 32
 // steps of the reduction, do not fit.  G keeps all its bits: it is split by truncation into 1 (bfloat16), 2 (half: 8 + 3 bits) or 3 (float32: 8 + 8 + 8 bits)
 // bfloat16 pieces with an exact sum.
-//   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; or 128 x 128, three stages ahead, with eight waves of 64 x 32 (one piece) or
-//     four of 64 x 64: a stage of the small tile is multiplied in a fifth of the time that memory takes to answer.  Stages of R rows (64; 32 with more than
-//     one piece) in LDS, read with the transpose load ds_read_b64_tr_b16.
+//   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; 128 x 128, three stages ahead, with eight waves of 64 x 32 (one piece) or
+//     four of 64 x 64; or 64 x 64 with four waves of 32 x 32: a stage of the small tiles is multiplied in a fifth of the time that memory takes to answer.  Stages of R rows (64; 32 with more than
+//     one piece in the larger tiles) in LDS, read with the transpose load ds_read_b64_tr_b16.
 //     The large tile is bound by LDS as much as by the products: 64 rows are 2048 clocks of matrix instructions, and 1536 of reads and 512 of writes in LDS.
 //   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
 //   * Of the two waves on a SIMD one multiplies a stage before it brings the next one into place, the other after it: the matrix cores work while operands are
 //     converted (16384 x 4096 x 4096: 459 -> 427 us; 37632 x 1024 x 1280: 183 -> 174).
 //   * Few tiles and many rows: the rows are split over workgroups, each stores its partial tile, and a second launch adds them in order.
 // LDS rows hold TW columns without padding (the DMA image is linear).  The transpose load reads 32 bytes of 16 rows, r = 8 q + 0 .. 3 (+ 4): the 32-byte
-// pairs of a row are XOR-swizzled with (r & 3) + 4 ((r >> 3) & 1), which spreads them over all banks.
+// pairs of a row are XOR-swizzled with (r & 3) + 4 ((r >> 3) & 1), which spreads them over all banks; 64 columns are four pairs, and two rows cover the banks, so
+// bits 1 and 3 of r do.
 #include "pack8.h"
 
 namespace {
@@ -46,7 +47,7 @@ template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 
     for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(u[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ int wg_swz(int row) { return (row & 3) | ((row >> 1) & 4); }
+template <int TW> __device__ __forceinline__ int wg_swz(int row) { return TW == 64 ? ((row >> 1) & 1) | ((row >> 2) & 2) : (row & 3) | ((row >> 1) & 4); }
 
 // WN x WK waves of (16 TN) x (16 TK); both sides of the tile are TW wide.  GDMA: G straight to LDS (P == 1, 16-byte aligned rows, MODE 0); otherwise through
 // registers (MODE: vec8.h).  Two forms:
@@ -60,7 +61,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   static_assert(WK * TK * 16 == TW, "square tiles");
   constexpr bool RING = NST > 2;
   static_assert(!GDMA || P == 1, "pieces come from registers");
-  constexpr int R = P == 1 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB;
+  constexpr int R = P == 1 || TW == 64 ? 64 : 32, ROWB = TW * 2, PLANE = R * ROWB;
   constexpr int XL = TW / 16, XR = NTH / XL, XP = R / XR;               // lanes of a row of codes (16 each), rows of a pass, passes
   constexpr int GL = TW / 8, GRW = NTH / GL, GP = R / GRW;              // the same for 8 gradients a lane
   constexpr int DW = RING ? NW : NW / 2, DI = GDMA ? PLANE / 1024 / DW : 0, RPI = 1024 / ROWB; // direct DMA: waves that issue it (large tile: those that multiply
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   int dcol[2];                                             // every other pass has the other half of the swizzle where a pass covers 8 rows
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int c = n0 + (((dslot >> 1) ^ wg_swz(drow + i * DW * RPI)) * 2 + (dslot & 1)) * 8;
+    const int c = n0 + (((dslot >> 1) ^ wg_swz<TW>(drow + i * DW * RPI)) * 2 + (dslot & 1)) * 8;
     dcol[i] = c < g.N ? c : g.N - 8;                       // columns behind the matrix: any (not stored)
   }
   const int xr = t / XL, xc = (t % XL) * 16;
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
         split8<P>(v, piece);
 #pragma unroll
         for (int p = 0; p < P; ++p)
-          *reinterpret_cast<uint4*>(sb + p * PLANE + r * ROWB + (((gc >> 4) ^ wg_swz(r)) << 5) + ((gc & 8) << 1)) = r < left ? piece[p] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(sb + p * PLANE + r * ROWB + (((gc >> 4) ^ wg_swz<TW>(r)) << 5) + ((gc & 8) << 1)) = r < left ? piece[p] : make_uint4(0, 0, 0, 0);
       }
     }
 #pragma unroll
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
         x.h[2 * j + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r < left ? c[j] : 0u, s, true);
       }
       // neighbouring lanes are 32 bytes apart: odd ones write their second half first, so that each instruction covers all banks
-      char* p = xplane(st) + r * ROWB + (((xc >> 4) ^ wg_swz(r)) << 5);
+      char* p = xplane(st) + r * ROWB + (((xc >> 4) ^ wg_swz<TW>(r)) << 5);
       const bool odd = t & 1;
       const uint4 u = x.u[0], v = x.u[1];                // (component by component: a choice between the two would put the array into scratch memory)
       *reinterpret_cast<uint4*>(p + (odd ? 16 : 0)) = make_uint4(odd ? v.x : u.x, odd ? v.y : u.y, odd ? v.z : u.z, odd ? v.w : u.w);
@@ -202,7 +203,7 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
 #pragma unroll
     for (int b = 0; b < TK; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   typedef s16x4_t __attribute__((address_space(3))) * lds_v4;
-  const int swz = wg_swz((lq << 3) + (li >> 2));         // of every row this lane reads
+  const int swz = wg_swz<TW>((lq << 3) + (li >> 2));         // of every row this lane reads
   const int rowo = (lq * 8 + (li >> 2)) * ROWB + (li & 3) * 8;
   auto trload = [&](const char* plane, int mc, int f) {  // 16-column tile f of the 32 rows mc: 8 rows of one column for each lane
     union { struct { s16x4_t lo, hi; } s; b16x8_t v; } u;
@@ -336,17 +337,14 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
   }
 }
 
-// dW (+)= the S partial products, in order: four columns a thread; partial rows hold a multiple of four
-__global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int S, long long plane, float* dW, long long ldw, int N, int K, int accumulate, int vec) {
+// dW (+)= the S partial products: four columns a thread, partial rows hold a multiple of four
+template <int GR> __global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int S, long long plane, float* dW, long long ldw, int N, int K, int accumulate, int vec) {
+  long long i;
+  float4 v;
+  if (!p8_sum_parts<GR>(part, S, plane, i, v)) return;
   const int q = (K + 3) >> 2;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n = i / q;
+  const long long n = i / q;
   const int k = (int)(i - n * q) * 4;
-  if (n >= N) return;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < S; ++s) {
-    const float4 x = *reinterpret_cast<const float4*>(part + s * plane + i * 4);
-    v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
-  }
   float* p = dW + n * ldw + k;
   if (vec && k + 4 <= K) {
     if (accumulate) { const float4 o = *reinterpret_cast<const float4*>(p); v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
@@ -358,21 +356,41 @@ __global__ __launch_bounds__(256) void wgrad8_join_kernel(const float* part, int
 }
 
 struct Split { int tile, S; long long rows; };
-// 256 x 256 tiles where at least 192 of them keep the compute units busy, otherwise 128 x 128 with the rows split for at least 256 workgroups, four
-// stages in each
-inline Split split_of(long long M, int N, int K) {
-  const long long t256 = (long long)((N + 255) / 256) * ((K + 255) / 256), t128 = (long long)((N + 127) / 128) * ((K + 127) / 128), stages = (M + 63) / 64;
-  if (t256 >= 192) return {256, 1, stages * 64};
-  long long S = 256 / t128;
-  if (S > stages / 4) S = stages / 4;
-  if (S < 1) S = 1;
-  const long long per = (stages + S - 1) / S;
-  return {128, (int)((stages + per - 1) / per), per * 64};
+// 256 x 256 tiles where at least 192 of them keep the compute units busy.  Otherwise 128 x 128 or 64 x 64, the rows split for about 256 workgroups with at
+// least four stages of 64 rows each, whichever is estimated to end first: a stage of one piece takes 0.85 or 0.62 us (0.85 for 64 x 64 too where two workgroups share a compute
+// unit), two and three pieces take one and a half times and twice as long, and partial products cost a launch of 3.5 us and their way out and back at 3.5 TB/s.
+// Measured in us, 128 against 64 (rows x N x K): 2352 x 1024 x 1280 26 / 34, 1024 x 1024 x 1024 19 / 13, 4096 x 1024 x 1024 30 / 42, 4096 x 512 x 512 20 / 17,
+// 300 x 1024 x 1024 10.4 / 6.6; f32 1024 x 1024 x 1024 28 / 21, 2352 x 1024 x 1280 47 / 80.
+inline Split split_of(int pieces, long long M, int N, int K) {
+  const long long stages = (M + 63) / 64;
+  if ((long long)((N + 255) / 256) * ((K + 255) / 256) >= 192) return {256, 1, stages * 64};
+  Split best = {0, 1, 0};
+  double least = 0;
+  for (int tile = 64; tile <= 128; tile += 64) {
+    const long long t = (long long)((N + tile - 1) / tile) * ((K + tile - 1) / tile);
+    long long S = 256 / t;
+    if (S > stages / 4) S = stages / 4;
+    if (S < 1) S = 1;
+    const long long per = (stages + S - 1) / S;
+    S = (stages + per - 1) / per;
+    const long long wgs = t * S;
+    const double stage = (tile == 64 ? (wgs <= 256 ? 0.62 : 0.85 * (double)((wgs + 511) / 512)) : 0.85 * (double)((wgs + 255) / 256)) * (1 + pieces) / 2;
+    const double us = (double)per * stage + (S > 1 ? 3.5 + (double)S * N * K * 8 / 3.5e6 : 0.);
+    if (best.tile == 0 || us < least) { best = {tile, (int)S, per * 64}; least = us; }
+  }
+  return best;
+}
+inline int pieces_of(int dtype) {
+#ifdef SPB_F16
+  return dtype == SPB_F32 ? 3 : 2;
+#else
+  return dtype == SPB_F32 ? 3 : 1;
+#endif
 }
 inline long long part_plane(int N, int K) { return (long long)N * ((K + 3) / 4 * 4); }
 
 template <typename T, int P, bool GDMA, int MODE, int NST, int WN, int WK, int TN, int TK> int launch(const Wgrad8Args& g, int S, hipStream_t s) {
-  constexpr int R = P == 1 ? 64 : 32, TW = WN * TN * 16, PLANE = R * TW * 2, NTH = WN * WK * 64;
+  constexpr int TW = WN * TN * 16, R = P == 1 || TW == 64 ? 64 : 32, PLANE = R * TW * 2, NTH = WN * WK * 64;
   constexpr int RING = NST > 2 ? NST * (R * TW + R * TW / 4) : 0;      // codes, a dword of scales a lane
   constexpr int LDS = ((GDMA ? NST : 2 * P) + 2) * PLANE + RING;
   static_assert(LDS <= 160 * 1024 && NTH * 16 <= R * TW, "fits a compute unit");
@@ -386,6 +404,7 @@ template <typename T, int P, bool GDMA, int MODE> int run(Wgrad8Args g, const Sp
   g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
   if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
   if (sp.tile == 256) return launch<T, P, GDMA, MODE, 2, 2, 4, 8, 4>(g, sp.S, s);
+  if (sp.tile == 64) return launch<T, P, GDMA, MODE, 4, 2, 2, 2, 2>(g, sp.S, s);
   if constexpr (P == 1) return launch<T, P, GDMA, MODE, 4, 2, 4, 4, 2>(g, sp.S, s);
   else return launch<T, P, GDMA, MODE, 4, 2, 2, 4, 4>(g, sp.S, s);
 }
@@ -404,7 +423,7 @@ __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long l
 extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
   if (M == 0 || N == 0 || K == 0) return 0;
-  const Split sp = split_of(M, N, K);
+  const Split sp = split_of(pieces_of(dtype), M, N, K);
   return sp.S > 1 ? (long long)sp.S * part_plane(N, K) * 4 : 0;
 }
 
@@ -422,7 +441,7 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
     return 0;
   }
   if (!a->G || !a->X || !a->Xs || ((uintptr_t)a->X & 15) || ((uintptr_t)a->Xs & 3)) return SPB_E_ARG;
-  const Split sp = split_of(a->M, a->N, a->K);
+  const Split sp = split_of(pieces_of(dtype), a->M, a->N, a->K);
   if (sp.S > 1 && (!a->ws || ((uintptr_t)a->ws & 15) || a->ws_bytes < spb_gemm8_wgrad_bytes(dtype, a->M, a->N, a->K))) return SPB_E_ARG;
   const long long plane = part_plane(a->N, a->K);
   const int outvec = ((uintptr_t)a->dW & 15) == 0 && a->ldw % 4 == 0;
@@ -439,8 +458,9 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
 #endif
   if (e) return e;
   if (sp.S > 1) {
-    hipLaunchKernelGGL(wgrad8_join_kernel, dim3((unsigned)((plane / 4 + 255) / 256)), dim3(256), 0, s, (const float*)a->ws, sp.S, plane, a->dW, a->ldw, a->N, a->K,
-                       a->accumulate, outvec);
+    const long long blocks = p8_join_blocks(plane, sp.S);
+    if (sp.S > P8_JOIN) hipLaunchKernelGGL((wgrad8_join_kernel<16>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)a->ws, sp.S, plane, a->dW, a->ldw, a->N, a->K, a->accumulate, outvec);
+    else hipLaunchKernelGGL((wgrad8_join_kernel<1>), dim3((unsigned)blocks), dim3(256), 0, s, (const float*)a->ws, sp.S, plane, a->dW, a->ldw, a->N, a->K, a->accumulate, outvec);
     SPB_CHECK_LAUNCH();
   }
   return 0;

@@ -284,6 +284,20 @@ def test_wgrad_of_every_tile(device, M, N, K, dtype):
     check_wgrad(G, X8, ops.gemm8_wgrad(G, X8, dW=before.clone()), before.double())
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["dense", "slab", "odd"])
+@pytest.mark.parametrize("M,N,K", [(5001, 133, 700), (4490, 1000, 264), (40000, 5, 2300), (9217, 72, 96), (300, 1030, 1100), (128, 40, 30), (129, 64, 200)])
+def test_wgrad_of_small_tiles(device, M, N, K, layout, dtype):
+    """128- and 64-wide tiles, whole and odd columns, one to many parts of the rows, ragged last stages"""
+    from speedplusbaseline_amd import ops
+    G, X8 = data(M, N, dtype, M, layout, scale=1e-3), ops.quant8(data(M, K, torch.bfloat16, N))
+    first = ops.gemm8_wgrad(G, X8)
+    check_wgrad(G, X8, first)
+    assert torch.equal(first, ops.gemm8_wgrad(G, X8))
+    before = torch.randn(N, K, device="cuda")
+    check_wgrad(G, X8, ops.gemm8_wgrad(G, X8, dW=before.clone()), before.double())
+
+
 def test_wgrad_keeps_all_bits_of_the_gradient(device):
     """one row: dW is the outer product, exact up to its own rounding"""
     from speedplusbaseline_amd import ops
