@@ -751,7 +751,7 @@ int spb_act8_fwd(int dtype, int act, const void* X, long long ldx, void* Y, long
 int spb_act8_bwd(int dtype, int act, const void* G, long long ldg, const unsigned char* codes, const unsigned char* scales, void* dX, long long ldd,
                  long long M, int K, spb_stream_t stream);
 
-/* ---- products of packed operands (csrc/gemm8.hip, csrc/wgrad8.hip); K <= 2^23 -----------------------------------------------------------------
+/* ---- products of packed operands (csrc/gemm8.hip, csrc/wgrad8.hip); K <= 2^23, N <= 2^30 --------------------------------------------------------
  * Y[m,n] = sum_k A[m,k] * B[n,k] + bias[n], accumulated in f32.  A is packed by rows, B by rows or by 128 x 128 blocks.
  * dtype SPB_BF16 (the library's 16-bit type): the 8-bit matrix instructions, which drop what lies below 2^-13 of the largest of 8 neighbouring
  * products (about 1.4e-5 of the result's rms on normal data, 4e-5 with outlier channels, whatever K; far below the output's rounding).
@@ -763,7 +763,7 @@ typedef struct spb_gemm8_args {
   const unsigned char* Bs; /* [N or ceil(N/128)][Sp] scales */
   const float* bias;       /* [N] or NULL */
   void* Y;                 /* [M,N], row stride ldy */
-  void* ws;                /* workspace of spb_gemm8_bytes(M, N, K) bytes, 16-byte aligned; may be NULL if that is 0 */
+  void* ws;                /* workspace of spb_gemm8_bytes(dtype, M, N, K) bytes, 16-byte aligned; may be NULL if that is 0 */
   long long ws_bytes;
   long long M, ldy;
   int N, K;
@@ -778,7 +778,7 @@ typedef struct spb_wgrad8_args {
   const unsigned char* X;  /* [M][Kp] codes */
   const unsigned char* Xs; /* [M][Sp] scales */
   float* dW;               /* [N,K], row stride ldw */
-  void* ws;                /* workspace of spb_gemm8_wgrad_bytes(M, N, K) bytes, 16-byte aligned; may be NULL if that is 0 */
+  void* ws;                /* workspace of spb_gemm8_wgrad_bytes(dtype, M, N, K) bytes, 16-byte aligned; may be NULL if that is 0 */
   long long ws_bytes;
   long long M, ldg, ldw;
   int N, K;

@@ -392,7 +392,7 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
 }  // namespace
 
 extern "C" long long spb_gemm8_bytes(int dtype, long long M, int N, int K) {
-  if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
+  if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || N > P8_SIDE_MAX || K < 0 || K > P8_DEPTH_MAX) return SPB_E_SHAPE;
   if (M <= ROWS_MAX || N == 0 || K == 0) return 0;
   const Cut c = cut_of(M, N, (K + 127) / 128);
   return c.S > 1 ? (long long)c.S * M * ((N + 3) / 4 * 4) * 4 : 0;
@@ -400,7 +400,7 @@ extern "C" long long spb_gemm8_bytes(int dtype, long long M, int N, int K) {
 
 extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stream) {
   if (!a || (dtype != SPB_F32 && dtype != SPB_BF16) || (a->b_block_rows != 1 && a->b_block_rows != 128)) return SPB_E_ARG;
-  if (a->M < 0 || a->N < 0 || a->K < 0 || a->K > (1 << 23) || (a->M > 1 && a->ldy < a->N)) return SPB_E_SHAPE;
+  if (a->M < 0 || a->N < 0 || a->N > P8_SIDE_MAX || a->K < 0 || a->K > P8_DEPTH_MAX || (a->M > 1 && a->ldy < a->N)) return SPB_E_SHAPE;
   if (a->M == 0 || a->N == 0) return 0;
   if (!a->Y) return SPB_E_ARG;
   hipStream_t s = (hipStream_t)stream;

@@ -6,6 +6,9 @@
 #define P8_E_LOW (-110)               // smallest / largest exponent of a scale: every value code * 2^e is then a normal bfloat16
 #define P8_E_HIGH 120
 
+#define P8_DEPTH_MAX (1 << 23)        // longest row of codes in a product: the rows of a tile are reached by 32-bit offsets
+#define P8_SIDE_MAX (1 << 30)         // most rows of B, columns of G: rounded up to a tile they fit an int
+
 static inline int p8_cols(int K) { return (K + 127) / 128 * 128; }          // Kp: bytes of a row of codes
 static inline int p8_scales(int K) { return ((K + 127) / 128 + 3) / 4 * 4; } // Sp: bytes of a row of scales
 

@@ -421,7 +421,7 @@ __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long l
 }  // namespace
 
 extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K) {
-  if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || K < 0) return SPB_E_SHAPE;
+  if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || N > P8_SIDE_MAX || K < 0 || K > P8_DEPTH_MAX) return SPB_E_SHAPE;
   if (M == 0 || N == 0 || K == 0) return 0;
   const Split sp = split_of(pieces_of(dtype), M, N, K);
   return sp.S > 1 ? (long long)sp.S * part_plane(N, K) * 4 : 0;
@@ -429,7 +429,7 @@ extern "C" long long spb_gemm8_wgrad_bytes(int dtype, long long M, int N, int K)
 
 extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream_t stream) {
   if (!a || (dtype != SPB_F32 && dtype != SPB_BF16)) return SPB_E_ARG;
-  if (a->M < 0 || a->N < 0 || a->K < 0 || a->K > (1 << 23) || a->ldg < 0 || (a->N > 1 && a->ldw < a->K)) return SPB_E_SHAPE;     // 64 rows of codes: 32-bit offsets
+  if (a->M < 0 || a->N < 0 || a->N > P8_SIDE_MAX || a->K < 0 || a->K > P8_DEPTH_MAX || a->ldg < 0 || (a->N > 1 && a->ldw < a->K)) return SPB_E_SHAPE;
   if (a->N == 0 || a->K == 0) return 0;
   if (!a->dW) return SPB_E_ARG;
   hipStream_t s = (hipStream_t)stream;

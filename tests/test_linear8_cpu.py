@@ -104,6 +104,14 @@ def test_product_refusals(lib):
     assert l.spb_gemm8_wgrad_bytes(1, 100000, 64, 256) > 0 and l.spb_gemm8_wgrad_bytes(1, 0, 64, 256) == 0 and l.spb_gemm8_wgrad_bytes(7, 1, 1, 1) < 0
 
 
+@pytest.mark.parametrize("lib", [L.lib, L.lib_f16], ids=["bf16", "f16"])
+def test_products_refuse_sides_that_do_not_fit_their_offsets(lib):
+    l, deep, wide = lib(), (1 << 23) + 1, (1 << 30) + 1
+    assert l.spb_gemm8(1, product(N=wide, ldy=wide), None) == SHAPE and l.spb_gemm8_wgrad(1, wgrad(N=wide, ldg=wide), None) == SHAPE
+    for f in (l.spb_gemm8_bytes, l.spb_gemm8_wgrad_bytes):
+        assert f(1, 100, wide, 128) == SHAPE and f(1, 100, 128, deep) == SHAPE and f(1, 100, wide - 1, 128) >= 0 and f(1, 100, 128, deep - 1) >= 0
+
+
 def test_argument_structs_have_the_layout_of_the_header(tmp_path):
     import os
     import subprocess
