@@ -345,7 +345,9 @@ constexpr long long ROWS_MAX = 16;
 // How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 211 us, 128 x 128: 261 us) but leave compute units idle below about 144 of
 // them (2816 x 4096 x 4096, 176 tiles: 49 against 54 us; 2048 x 4096 x 2048, 128 tiles: 28 against 22 us).  128 x 128 tiles are used down to as many
 // (2352 x 1024 x 1024, 152 tiles: 8.4 us, 64 x 64: 10.1; 2048 x 1024 x 1024, 128 tiles: 8.3 and 7.0).  Smaller products take 64 x 64 tiles, and where
-// even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up.
+// even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
+// worth that launch (3.5 us) and the partial sums' way out and back at 3.5 TB/s: 48 x 4096 x 9216 in four parts 12.4 us, in one 21.7, 300 x 512 x 4096 9.3 and
+// 11.1, but 4096 x 128 x 1024 in two parts 9.2, in one 5.1.
 struct Cut { int tile, S, steps; };
 inline Cut cut_of(long long M, int N, int KT) {
   const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
@@ -354,8 +356,10 @@ inline Cut cut_of(long long M, int N, int KT) {
   long long S = t64 >= 256 ? 1 : 256 / t64;
   const int quads = (KT + 3) / 4;
   if (S > quads) S = quads;
-  const int per = (int)((quads + S - 1) / S);
-  return {64, (quads + per - 1) / per, per * 4};
+  int per = (int)((quads + S - 1) / S);
+  S = (quads + per - 1) / per;
+  if (S > 1 && (quads - per) * 4 * 0.29 < 3.5 + (double)S * (double)M * N * 8 / 3.5e6) { per = quads; S = 1; }
+  return {64, (int)S, per * 4};
 }
 template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hipStream_t s) {
   if (g.M <= ROWS_MAX) {
