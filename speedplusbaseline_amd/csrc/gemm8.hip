@@ -244,7 +244,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const long long m = m0 + (wm * TM + i) * 16 + li;
-      if (m < g.M) put<V, TO>(g, Y, m, n, &acc[i][j], bias);
+      if (m >= g.M) continue;
+      if constexpr (V == 4) {
+        if (g.plane) {
+          if (n < g.ldy) p8_put_part(reinterpret_cast<float*>(Y) + m * g.ldy + n, acc[i][j]);
+          continue;
+        }
+      }
+      put<V, TO>(g, Y, m, n, &acc[i][j], bias);
     }
   }
 }

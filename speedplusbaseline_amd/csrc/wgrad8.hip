@@ -324,7 +324,9 @@ __global__ __launch_bounds__(WN * WK * 64) void wgrad8_kernel(const Wgrad8Args g
       const int k = k0 + (wk * TK + b) * 16 + lq * 4;
       float* p = out + (long long)n * g.ldo + k;
       f32x4_t v = acc[a][b];
-      if (g.vec && k + 4 <= g.K) {
+      if (g.plane) {
+        if (k < g.ldo) p8_put_part(p, v);
+      } else if (g.vec && k + 4 <= g.K) {
         float4 o = make_float4(v[0], v[1], v[2], v[3]);
         if (g.accumulate) { const float4 q = *reinterpret_cast<const float4*>(p); o.x += q.x; o.y += q.y; o.z += q.z; o.w += q.w; }
         *reinterpret_cast<float4*>(p) = o;
@@ -446,7 +448,7 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
   const long long plane = part_plane(a->N, a->K);
   const int outvec = ((uintptr_t)a->dW & 15) == 0 && a->ldw % 4 == 0;
   const Wgrad8Args g = {a->G, a->X, a->Xs, sp.S > 1 ? (float*)a->ws : a->dW, a->M, a->ldg, sp.S > 1 ? plane / a->N : a->ldw, sp.S > 1 ? plane : 0, sp.rows, a->N, a->K,
-                        p8_cols(a->K), p8_scales(a->K), 0, 0, sp.S > 1 ? 0 : a->accumulate, sp.S > 1 ? 1 : outvec};
+                        p8_cols(a->K), p8_scales(a->K), 0, 0, sp.S > 1 ? 0 : a->accumulate, outvec};
   int e;
   if (dtype == SPB_F32) e = run_regs<float, 3>(g, sp, s);
 #ifdef SPB_F16
