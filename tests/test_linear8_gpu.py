@@ -482,3 +482,66 @@ def test_two_products_at_once_share_nothing(device):
     for i in range(2):
         for y, dw in got[i]:
             assert torch.equal(y, sets[i][4]) and torch.equal(dw, sets[i][5])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(3000, 3333, 130), (3700, 1300, 130), (2100, 1111, 260), (300, 333, 700), (40, 130, 9100), (17, 30, 17000), (5, 77, 300)])
+def test_products_of_every_tile_into_odd_columns(device, M, N, K, dtype):
+    """the vectors of a result go to any address; what stands beside it stays"""
+    from speedplusbaseline_amd import ops
+    A, (B, _), bias = ops.quant8(data(M, K, dtype, 1)), ops.quant8_weight(data(N, K, torch.float32, 2)), torch.randn(N, device="cuda")
+    want = ops.gemm8(A, B, bias=bias, dtype=dtype)
+    for off, width in ((3, N + 6), (1, N + 9)):
+        wide = torch.full((M, width), 7.0, dtype=dtype, device="cuda")
+        y = ops.gemm8(A, B, bias=bias, dtype=dtype, Y=wide[:, off:off + N])
+        assert torch.equal(y, want) and (wide[:, :off] == 7).all() and (wide[:, off + N:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(70, 3500, 3593), (5001, 136, 701), (129, 66, 203)])
+def test_wgrad_of_every_tile_into_odd_columns(device, M, N, K, dtype):
+    from speedplusbaseline_amd import ops
+    G, X8 = data(M, N, dtype, M, scale=1e-3), ops.quant8(data(M, K, torch.bfloat16, N))
+    want = ops.gemm8_wgrad(G, X8)
+    wide = torch.zeros(N, K + 6, device="cuda")
+    wide[:, :3], wide[:, 3 + K:] = 7, 7
+    assert torch.equal(ops.gemm8_wgrad(G, X8, dW=wide[:, 3:3 + K]), want) and (wide[:, :3] == 7).all() and (wide[:, 3 + K:] == 7).all()
+
+
+def test_broadcast_rows_and_separate_buffers(device):
+    """operands with a row stride of 0, a packed matrix made of one's own tensors, one operand twice"""
+    from speedplusbaseline_amd import _lib as L, ops
+    for dtype in TYPES:
+        row = data(1, 264, dtype, 5)
+        rows = row.expand(300, 264)
+        P, Q = ops.quant8(rows), ops.quant8(rows.contiguous())
+        assert torch.equal(P.codes, Q.codes) and torch.equal(P.scales, Q.scales)
+        W, V = ops.quant8_weight(rows), ops.quant8_weight(rows.contiguous())
+        assert all(torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) for a, b in zip(W, V))
+        own = ops.Packed8(Q.codes.clone(), Q.scales.clone(), 264, 1)
+        assert torch.equal(ops.gemm8(own, own, dtype=dtype), ops.gemm8(Q, Q, dtype=dtype)) and torch.equal(ops.dequant8(own), ops.dequant8(Q))
+        for g in (rows, rows[:, :136], rows[:, 1:120]):
+            assert torch.equal(ops.gemm8_wgrad(g, own), ops.gemm8_wgrad(g.contiguous(), Q))
+        y, R = ops.act8_fwd(rows, L.ACT_GELU)
+        z, S = ops.act8_fwd(rows.contiguous(), L.ACT_GELU)
+        assert torch.equal(y, z) and torch.equal(R.codes, S.codes)
+        assert torch.equal(ops.act8_bwd(rows, R, L.ACT_GELU), ops.act8_bwd(rows.contiguous(), S, L.ACT_GELU))
+
+
+def test_split_products_in_a_graph(device):
+    """many parts and their sums, captured, replayed on changing inputs beside eager work"""
+    from speedplusbaseline_amd import ops
+    x, G = data(40, 9100, torch.bfloat16, 1), data(9000, 40, torch.bfloat16, 2)
+    B, X8 = ops.quant8_weight(data(70, 9100, torch.float32, 3))[0], ops.quant8(data(9000, 24, torch.bfloat16, 4))
+    xs, gs = x.clone(), G.clone()
+    ops.gemm8(ops.quant8(xs), B), ops.gemm8_wgrad(gs, X8)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dw = ops.gemm8(ops.quant8(xs), B), ops.gemm8_wgrad(gs, X8)
+    for i in range(4):
+        xs.copy_(x * (i + 1)), gs.copy_(G.flip(0) if i % 2 else G)
+        want = ops.gemm8(ops.quant8(xs), B), ops.gemm8_wgrad(gs, X8)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(dw, want[1]), i
