@@ -325,7 +325,7 @@ def fc_wgrad_update(gT, xT, M, kind, params, grads=None, m=None, v=None, gmul=No
 # Operands are 2-D with contiguous columns and any row stride.  Like every function of this file they enqueue on the current stream and build no
 # autograd graph: the backward pass is the explicit *_bwd / *_wgrad call.  They run on the device of their tensors, whichever is current.
 # A call on a few rows is bound by this file, not by its kernel (12-22 us with the helpers above; like this quant8 and gemm8 take 7 us, layernorm_bwd with
-# its five tensors and two launches 17 us): devices are compared as indices, argument structs are filled by position, and addresses are plain integers.
+# its five tensors and two launches 16 us): devices are compared as indices, argument structs are filled by position, and addresses are plain integers.
 
 _TUNED = bool(os.environ.get("SPB_DEBUG") or os.environ.get("SPB_TUNING_LIB"))
 
@@ -337,7 +337,7 @@ def _lib8(dtype):
 
 
 def _call(dev, fn, what, *args):
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))     # current_stream(dev).cuda_stream without the 3 us of its object
         if code:
             L.check(code, what)
@@ -419,16 +419,17 @@ def layernorm_bwd(G, X, mean, rstd, gamma=None, dgamma=None, dbeta=None, dX=None
     else:
         ldd = _out(dX, (M, Cn), X.dtype, "dX", dev)
     lib = _lib8(X.dtype)
-    cap, part, accumulate = 0, None, 0
+    cap, part, accumulate, dgp, dbp = 0, None, 0, None, None
     if param_grads:
-        accumulate = 0 if dgamma is None else 1
         if dgamma is None:
             dgamma, dbeta = torch.empty((2, Cn), dtype=torch.float32, device=X.device).unbind(0)
+            dgp, dbp = dgamma.data_ptr(), dbeta.data_ptr()
+        else:
+            accumulate, dgp, dbp = 1, _vec(dgamma, Cn, "dgamma", dev), _vec(dbeta, Cn, "dbeta", dev)
         cap = lib.spb_layernorm_bwd_floats(M, Cn)
         part = torch.empty(cap, dtype=torch.float32, device=X.device)
     a = A8.LayerNormArgs(X.data_ptr(), G.data_ptr(), _vec(gamma, Cn, "gamma", dev), None, dX.data_ptr(), _vec(mean, M, "mean", dev),
-                         _vec(rstd, M, "rstd", dev), _vec(dgamma, Cn, "dgamma", dev), _vec(dbeta, Cn, "dbeta", dev),
-                         None if part is None else part.data_ptr(), cap, M, ldx, ldg, ldd, Cn, 0.0, accumulate)
+                         _vec(rstd, M, "rstd", dev), dgp, dbp, None if part is None else part.data_ptr(), cap, M, ldx, ldg, ldd, Cn, 0.0, accumulate)
     _call(dev, lib.spb_layernorm_bwd, "spb_layernorm_bwd", code, C.byref(a))
     return dX, dgamma, dbeta
 
