@@ -74,7 +74,10 @@ template <int GR> __device__ __forceinline__ bool p8_sum_parts(const float* part
   for (int s = s0; s < s1; s += B) {
     float4 x[B];
 #pragma unroll
-    for (int k = 0; k < B; ++k) x[k] = *reinterpret_cast<const float4*>(p + (s + k < s1 ? s + k : s1 - 1) * plane);
+    for (int k = 0; k < B; ++k) {
+      const f32x4_t q = s + k < s1 ? __builtin_nontemporal_load(reinterpret_cast<const f32x4_t*>(p + (s + k) * plane)) : (f32x4_t){0.f, 0.f, 0.f, 0.f};
+      x[k] = make_float4(q[0], q[1], q[2], q[3]);
+    }
 #pragma unroll
     for (int k = 0; k < B; ++k)
       if (s + k < s1) { v.x += x[k].x; v.y += x[k].y; v.z += x[k].z; v.w += x[k].w; }
