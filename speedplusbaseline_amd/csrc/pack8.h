@@ -57,12 +57,12 @@ __device__ __forceinline__ void dma4s(const void* sbase, unsigned voff, unsigned
                : "=&s"(keep) : "v"(voff), "s"(sbase), "s"(lds_base) : "memory");
 }
 
-// Sum of S partial planes in a fixed order, four neighbouring floats a thread (`i` is their number).  GR 1: a thread adds all of them, four requested at a time.
-// Many planes (S > P8_JOIN): GR threads take a part of the planes each, whose sums meet in LDS; one of them returns true with the result.
-constexpr int P8_JOIN = 16;
 // Four floats of a partial product past the caches: the next launch reads them on other XCDs, and lines left dirty in this one's L2 would be written back before
 // it could start (weight gradient 2352 x 1024 x 1280: 26.8 -> 23.8 us).
 __device__ __forceinline__ void p8_put_part(float* p, const f32x4_t& v) { __builtin_nontemporal_store(v, reinterpret_cast<f32x4_t*>(p)); }
+// Sum of S partial planes in a fixed order, four neighbouring floats a thread (`i` is their number).  GR 1: a thread adds all of them, four requested at a time.
+// Many planes (S > P8_JOIN): GR threads take a part of the planes each, whose sums meet in LDS; one of them returns true with the result.
+constexpr int P8_JOIN = 16;
 template <int GR> __device__ __forceinline__ bool p8_sum_parts(const float* part, int S, long long plane, long long& i, float4& v) {
   constexpr int Q = 256 / GR;
   const int ql = threadIdx.x % Q, gr = threadIdx.x / Q, per = (S + GR - 1) / GR, s0 = gr * per, s1 = s0 + per < S ? s0 + per : S;

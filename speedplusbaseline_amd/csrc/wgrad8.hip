@@ -6,8 +6,8 @@
 // steps of the reduction, do not fit.  G keeps all its bits: it is split by truncation into 1 (bfloat16), 2 (half: 8 + 3 bits) or 3 (float32: 8 + 8 + 8 bits)
 // bfloat16 pieces with an exact sum.
 //   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; 128 x 128, three stages ahead, with eight waves of 64 x 32 (one piece) or
-//     four of 64 x 64; or 64 x 64 with four waves of 32 x 32: a stage of the small tiles is multiplied in a fifth of the time that memory takes to answer.  Stages of R rows (64; 32 with more than
-//     one piece in the larger tiles) in LDS, read with the transpose load ds_read_b64_tr_b16.
+//     four of 64 x 64; or 64 x 64 with four waves of 32 x 32: a stage of the small tiles is multiplied in a fifth of the time that memory takes to answer.
+//     Stages of R rows (64; 32 with more than one piece in the larger tiles) in LDS, read with the transpose load ds_read_b64_tr_b16.
 //     The large tile is bound by LDS as much as by the products: 64 rows are 2048 clocks of matrix instructions, and 1536 of reads and 512 of writes in LDS.
 //   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
 //   * Of the two waves on a SIMD one multiplies a stage before it brings the next one into place, the other after it: the matrix cores work while operands are
@@ -359,8 +359,9 @@ template <int GR> __global__ __launch_bounds__(256) void wgrad8_join_kernel(cons
 
 struct Split { int tile, S; long long rows; };
 // 256 x 256 tiles where at least 192 of them keep the compute units busy.  Otherwise 128 x 128 or 64 x 64, the rows split for about 256 workgroups with at
-// least four stages of 64 rows each, whichever is estimated to end first: a stage of one piece takes 0.85 or 0.62 us (0.85 for 64 x 64 too where two workgroups share a compute
-// unit), two and three pieces take one and a half times and twice as long, and partial products cost a launch of 3.5 us and their way out and back at 3.5 TB/s.
+// least four stages of 64 rows each, whichever is estimated to end first: a stage of one piece takes 0.85 or 0.62 us (0.85 for 64 x 64 too where two workgroups
+// share a compute unit), two and three pieces take one and a half times and twice as long, and partial products cost a launch of 3.5 us and their way out and
+// back at 3.5 TB/s.
 // Measured in us, 128 against 64 (rows x N x K): 2352 x 1024 x 1280 26 / 34, 1024 x 1024 x 1024 19 / 13, 4096 x 1024 x 1024 30 / 42, 4096 x 512 x 512 20 / 17,
 // 300 x 1024 x 1024 10.4 / 6.6; f32 1024 x 1024 x 1024 28 / 21, 2352 x 1024 x 1280 47 / 80.
 inline Split split_of(int pieces, long long M, int N, int K) {
