@@ -233,3 +233,25 @@ def test_rows_behind_two_to_the_32(device):
     dx, dg, db = ops.layernorm_bwd(x, x, mean, rstd, dX=y)
     want = ops.layernorm_bwd(tail, tail, mean[-4:].contiguous(), rstd[-4:].contiguous())
     assert torch.equal(dx[-4:], want[0]) and torch.allclose(db, want[2], rtol=1e-6, atol=1e-6)
+
+
+def test_rows_behind_two_to_the_32(device):
+    """2.6e9 elements in place: the last rows as in a call of their own, forward and backward"""
+    from speedplusbaseline_amd import ops
+    M, C, last = 640000, 4096, 64
+    tail, g = rows_of(last, C, torch.bfloat16, 1), rows_of(last, C, torch.bfloat16, 2)
+    gamma = torch.randn(C, device="cuda")
+    want, mean, rstd = ops.layernorm_fwd(tail, gamma)
+    dx, dg, db = ops.layernorm_bwd(g, tail, mean, rstd, gamma)
+    X = torch.zeros(M, C, dtype=torch.bfloat16, device="cuda")
+    X[-last:] = tail
+    G = torch.zeros_like(X)
+    G[-last:] = g
+    y, m, r = ops.layernorm_fwd(X, gamma)
+    assert torch.equal(y[-last:], want) and torch.equal(m[-last:], mean) and torch.equal(r[-last:], rstd) and (y[:last] == 0).all()
+    d, dgamma, dbeta = ops.layernorm_bwd(G, X, m, r, gamma, dX=G)
+    assert torch.equal(d[-last:], dx) and (d[:last] == 0).all()
+    # the sums over rows: the same 64 terms in another order
+    top = lambda t: 70 * U * t.abs().sum(0)
+    xh = (tail.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    assert ((dgamma.double() - dg.double()).abs() <= top(g.double() * xh) * 2).all() and ((dbeta.double() - db.double()).abs() <= top(g.double()) * 2).all()

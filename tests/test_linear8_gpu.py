@@ -545,3 +545,20 @@ def test_split_products_in_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want[0]) and torch.equal(dw, want[1]), i
+
+
+def test_rows_behind_two_to_the_32(device):
+    """gradients, activations and checkpoints of 2.6e9 elements: the last rows as in a call of their own"""
+    from speedplusbaseline_amd import _lib as L, ops
+    M, N, last = 640000, 4096, 64
+    tail = data(last, N, torch.bfloat16, 1)
+    G = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+    G[-last:] = tail
+    x = data(last, 160, torch.bfloat16, 2)
+    X8 = ops.quant8(x.repeat(M // last, 1))
+    assert torch.equal(ops.gemm8_wgrad(G, X8), ops.gemm8_wgrad(tail, ops.quant8(x)))
+    y, P = ops.act8_fwd(G, L.ACT_SILU, Y=G)
+    want, Q = ops.act8_fwd(tail, L.ACT_SILU)
+    assert torch.equal(y[-last:], want) and torch.equal(P.codes[-last:], Q.codes) and (y[:last] == 0).all()
+    d = ops.act8_bwd(G, P, L.ACT_SILU, dX=G)
+    assert torch.equal(d[-last:], ops.act8_bwd(want, Q, L.ACT_SILU))
