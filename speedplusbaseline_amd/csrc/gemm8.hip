@@ -78,8 +78,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int TILE = (BM + BN) * 128, STAGE = TILE + (BM + BN) * 4;   // codes, then the dword of scales that holds this step's
   // Eight waves: the upper four, one on each SIMD, fetch at the head of a step, while the other four, whose instructions go first, multiply.  (All eight
-  // fetching between their products: 8192 x 8192 x 8192 419 us, like this 381; a wave that waits for a DMA instruction to be taken issues no product.)
-  constexpr bool LEAD = !EXACT && NW == 8;
+  // fetching between their products: 8192 x 8192 x 8192 419 us, like this 381; f32 16384 x 4096 x 4096 482 and 432; a wave that waits for a DMA instruction to be taken issues no product.)
+  constexpr bool LEAD = NW == 8;
   constexpr int DW = LEAD ? NW / 2 : NW, DI = (BM + BN) / 8 / DW;       // waves that fetch; DMA instructions of a stage for each: 8 rows of codes
   constexpr int ST = (BM + BN) / 64, SI = (ST + DW - 1) / DW;           // and 64 rows of scales each (a wave too many repeats an instruction)
   static_assert(DI * 8 * DW == BM + BN && ST * 64 == BM + BN, "whole DMA instructions");
@@ -207,29 +207,39 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm8_kernel(const Gemm8Args g) 
       }
     }
   } else {
+    // B's values of a step are converted once, A's a row tile at a time, while the one before is multiplied
+    if (LEAD && w >= DW) __builtin_amdgcn_s_setprio(1);
     for (int kt = 0; kt < KT; ++kt) {
       if (kt > 0) land(kt);
       if (kt + NST - 1 < KT) issue(kt + NST - 1, buf == 0 ? NST - 1 : buf - 1);
       const char* stage = smem + buf * STAGE;
       buf = buf == NST - 1 ? 0 : buf + 1;
-      i32x8_t b[TN], a[TM];
-      float fa[TM], fb[TN];
       const int sh = (kt & 3) * 8;
+      i32x8_t a[2];
+      float fa[2];
+      b16x8_t wb[TN][4];
+      a[0] = frag(stage + ao);
+      fa[0] = scale_of(*reinterpret_cast<const unsigned*>(stage + ato) >> sh);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) { b[j] = frag(stage + bo + brow(j) * 128); fb[j] = scale_of(*reinterpret_cast<const unsigned*>(stage + bto + brow(j) * 4) >> sh); }
+      for (int j = 0; j < TN; ++j) {
+        const i32x8_t b = frag(stage + bo + brow(j) * 128);
+        const float fb = scale_of(*reinterpret_cast<const unsigned*>(stage + bto + brow(j) * 4) >> sh);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) { a[i] = frag(stage + ao + i * 2048); fa[i] = scale_of(*reinterpret_cast<const unsigned*>(stage + ato + i * 64) >> sh); }
+        for (int h = 0; h < 4; ++h) wb[j][h] = wide8(b, h, fb);
+      }
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        b16x8_t wb[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) wb[j] = wide8(b[j], h, fb[j]);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const b16x8_t wa = wide8(a[i], h, fa[i]);
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], wa, acc[i][j], 0, 0, 0);
+      for (int i = 0; i < TM; ++i) {
+        if (i + 1 < TM) {
+          a[(i + 1) & 1] = frag(stage + ao + (i + 1) * 2048);
+          fa[(i + 1) & 1] = scale_of(*reinterpret_cast<const unsigned*>(stage + ato + (i + 1) * 64) >> sh);
         }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const b16x8_t wa = wide8(a[i & 1], h, fa[i & 1]);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j][h], wa, acc[i][j], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -350,15 +360,15 @@ template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int 
 
 constexpr long long ROWS_MAX = 16;
 // How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 211 us, 128 x 128: 261 us) but leave compute units idle below about 144 of
-// them (2816 x 4096 x 4096, 176 tiles: 49 against 54 us; 2048 x 4096 x 2048, 128 tiles: 28 against 22 us).  128 x 128 tiles are used down to as many
-// (2352 x 1024 x 1024, 152 tiles: 8.4 us, 64 x 64: 10.1; 2048 x 1024 x 1024, 128 tiles: 8.3 and 7.0).  Smaller products take 64 x 64 tiles, and where
-// even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
+// them (2816 x 4096 x 4096, 176 tiles: 49 against 54 us; 2048 x 4096 x 2048, 128 tiles: 28 against 22 us; f32 below about 192:
+// 2816 x 4096 x 1024 44 against 39 us).  128 x 128 tiles are used down to 144 of those (2352 x 1024 x 1024, 152 tiles: 8.4 us, 64 x 64: 10.1;
+// 2048 x 1024 x 1024, 128 tiles: 8.3 and 7.0).  Smaller products take 64 x 64 tiles, and where even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
 // worth that launch (3.5 us) and the partial sums' way out and back at 3.5 TB/s: 48 x 4096 x 9216 in four parts 12.4 us, in one 21.7, 300 x 512 x 4096 9.3 and
 // 11.1, but 4096 x 128 x 1024 in two parts 9.2, in one 5.1.
 struct Cut { int tile, S, steps; };
-inline Cut cut_of(long long M, int N, int KT) {
+inline Cut cut_of(bool exact, long long M, int N, int KT) {
   const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
-  if (t256 >= 144) return {256, 1, (KT + 3) / 4 * 4};
+  if (t256 >= (exact ? 192 : 144)) return {256, 1, (KT + 3) / 4 * 4};
   if (t128 >= 144) return {128, 1, (KT + 3) / 4 * 4};
   long long S = t64 >= 256 ? 1 : 256 / t64;
   const int quads = (KT + 3) / 4;
@@ -374,17 +384,15 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
     SPB_CHECK_LAUNCH();
     return 0;
   }
-  const Cut c = cut_of(g.M, g.N, g.Kp >> 7);
+  const Cut c = cut_of(EXACT, g.M, g.N, g.Kp >> 7);
   Gemm8Args h = g;
   h.steps = c.steps;
-  if constexpr (!EXACT) {
-    if (c.tile == 256) return run<256, 256, 2, 4, 2, false, TO>(h, 1, s);
-  }
+  if (c.tile == 256) return run<256, 256, 2, 4, 2, EXACT, TO>(h, 1, s);
   if (c.tile >= 128) {
-    // more tiles than compute units: two workgroups on each cover each other's waits (3840 x 2048 x 2048: 25.6 -> 22.1 us); fewer: four stages do (4096 x 1024 x 4096: 26.7 -> 24.4)
-    if constexpr (EXACT) return run<128, 128, 2, 2, 2, true, TO>(h, 1, s);
-    else if ((g.M + 127) / 128 * ((g.N + 127) / 128) > 256) return run<128, 128, 2, 4, 2, false, TO>(h, 1, s);
-    else return run<128, 128, 2, 4, 4, false, TO>(h, 1, s);
+    // more tiles than compute units: two workgroups on each cover each other's waits (3840 x 2048 x 2048: 25.6 -> 22.1 us); fewer: eight waves and four
+    // stages do (4096 x 1024 x 4096: 26.7 -> 24.4 us; f32 2352 x 1024 x 1024 17.1 -> 16.2).  f32 in two workgroups: four waves convert less (45.6 -> 43.4 us).
+    if ((g.M + 127) / 128 * ((g.N + 127) / 128) > 256) return run<128, 128, 2, EXACT ? 2 : 4, 2, EXACT, TO>(h, 1, s);
+    return run<128, 128, 2, 4, 4, EXACT, TO>(h, 1, s);
   }
   if (c.S == 1) return run<64, 64, 2, 2, 4, EXACT, TO>(h, 1, s);
   const long long q = (g.N + 3) / 4;
@@ -405,7 +413,7 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
 extern "C" long long spb_gemm8_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || N > P8_SIDE_MAX || K < 0 || K > P8_DEPTH_MAX) return SPB_E_SHAPE;
   if (M <= ROWS_MAX || N == 0 || K == 0) return 0;
-  const Cut c = cut_of(M, N, (K + 127) / 128);
+  const Cut c = cut_of(dtype == SPB_F32, M, N, (K + 127) / 128);
   return c.S > 1 ? (long long)c.S * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
