@@ -436,8 +436,9 @@ def layernorm_bwd(G, X, mean, rstd, gamma=None, dgamma=None, dbeta=None, dX=None
 
 class Packed8:
     """A matrix in e4m3 codes with one power-of-two scale for each block of 128 (include/spb_hip.h "8-bit packing"): codes uint8 [rows, K rounded up to
-    128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight)."""
-    __slots__ = ("K", "block_rows", "shape", "_rows", "_dev", "_own", "_qp", "_sp")
+    128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight).  Copies (copy, pickle, torch.save) hold their own tensors: device
+    and addresses are those of `_own` at the time of a call, never kept beside it."""
+    __slots__ = ("K", "block_rows", "shape", "_rows", "_own")
 
     def __init__(self, codes, scales, K, block_rows):
         kb = (K + 127) // 128
@@ -447,8 +448,8 @@ class Packed8:
         for t, shape in ((codes, (rows, kb * 128)), (scales, ((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4))):
             if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
                 raise RuntimeError("Packed8: codes and scales do not fit a packed [%d, %d] matrix" % (rows, K))
-        self.K, self.block_rows, self.shape, self._rows, self._dev = K, block_rows, (rows, K), rows, codes.get_device()
-        self._own, self._qp, self._sp = (codes, scales), codes.data_ptr(), scales.data_ptr()
+        self.K, self.block_rows, self.shape, self._rows = K, block_rows, (rows, K), rows
+        self._own = codes, scales
 
     @staticmethod
     def empty(rows, K, block_rows, device):
@@ -456,28 +457,33 @@ class Packed8:
         kb = (K + 127) // 128
         buf = torch.empty(rows * kb * 128 + (rows + block_rows - 1) // block_rows * ((kb + 3) // 4 * 4), dtype=torch.uint8, device=device)
         self = Packed8.__new__(Packed8)
-        self.K, self.block_rows, self.shape, self._rows, self._dev = K, block_rows, (rows, K), rows, buf.get_device()
-        self._own, self._qp = buf, buf.data_ptr()
-        self._sp = self._qp + rows * kb * 128
+        self.K, self.block_rows, self.shape, self._rows = K, block_rows, (rows, K), rows
+        self._own = (buf,)
         return self
 
     @property
     def device(self):
-        return (self._own if isinstance(self._own, torch.Tensor) else self._own[0]).device
+        return self._own[0].device
 
     @property
     def codes(self):
-        if isinstance(self._own, tuple):
+        if len(self._own) == 2:
             return self._own[0]
         kp = (self.K + 127) // 128 * 128
-        return self._own[:self._rows * kp].view(self._rows, kp)
+        return self._own[0][:self._rows * kp].view(self._rows, kp)
 
     @property
     def scales(self):
-        if isinstance(self._own, tuple):
+        if len(self._own) == 2:
             return self._own[1]
         kb = (self.K + 127) // 128
-        return self._own[self._rows * kb * 128:].view((self._rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4)
+        return self._own[0][self._rows * kb * 128:].view((self._rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4)
+
+    def _at(self):
+        """addresses of the codes and the scales"""
+        own = self._own
+        q = own[0].data_ptr()
+        return q, (own[1].data_ptr() if len(own) == 2 else q + self._rows * ((self.K + 127) // 128) * 128)
 
 
 def _packed(P, name, dev=None, block_rows=None):
@@ -486,16 +492,17 @@ def _packed(P, name, dev=None, block_rows=None):
         raise RuntimeError("%s must be a Packed8 (quant8 / quant8_weight), got %s" % (name, type(P).__name__))
     if block_rows is not None and P.block_rows != block_rows:
         raise RuntimeError("%s must be packed in blocks of %d x 128" % (name, block_rows))
-    if P._dev < 0 or (dev is not None and P._dev != dev):
+    on = P._own[0].get_device()
+    if on < 0 or (dev is not None and on != dev):
         raise RuntimeError("%s is on %s, expected %s" % (name, P.device, "a GPU" if dev is None else "device %d" % dev))
-    return P._dev
+    return on
 
 
 def quant8(X):
     """X [M, K] packed in blocks of 1 x 128: operand of gemm8 and checkpoint for gemm8_wgrad"""
     dev, M, K, ldx, code = _mat(X, "X")
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, P._qp, P._sp)
+    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, *P._at())
     return P
 
 
@@ -504,8 +511,8 @@ def quant8_weight(W, transpose=True):
     dev, N, K, ldw, code = _mat(W, "W")
     P = Packed8.empty(N, K, 128, W.device)
     T = Packed8.empty(K, N, 128, W.device) if transpose else None
-    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, P._qp, P._sp,
-          T._qp if transpose else None, T._sp if transpose else None)
+    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, *P._at(),
+          *(T._at() if transpose else (None, None)))
     return P, T
 
 
@@ -515,7 +522,7 @@ def dequant8(P, dtype=torch.bfloat16, Y=None):
     if Y is None:
         Y = torch.empty(P.shape, dtype=dtype, device=P.device)
     ldy = _out(Y, P.shape, dtype, "Y", dev)
-    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], P._qp, P._sp, P.block_rows, P._rows, P.K, Y.data_ptr(), ldy)
+    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], *P._at(), P.block_rows, P._rows, P.K, Y.data_ptr(), ldy)
     return Y
 
 
@@ -536,7 +543,7 @@ def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
     lib, code = _lib8(dtype), _DT[dtype]
     need = lib.spb_gemm8_bytes(code, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=A.device) if need > 0 else None
-    a = A8.Gemm8Args(A._qp, A._sp, B._qp, B._sp, _vec(bias, N, "bias", dev), Y.data_ptr(),
+    a = A8.Gemm8Args(*A._at(), *B._at(), _vec(bias, N, "bias", dev), Y.data_ptr(),
                      None if ws is None else ws.data_ptr(), need, M, ldy, N, K, B.block_rows)
     _call(dev, lib.spb_gemm8, "spb_gemm8", code, C.byref(a))
     return Y
@@ -557,7 +564,7 @@ def gemm8_wgrad(G, X8, dW=None):
     lib = _lib8(G.dtype)
     need = lib.spb_gemm8_wgrad_bytes(code, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=G.device) if need > 0 else None
-    a = A8.Wgrad8Args(G.data_ptr(), X8._qp, X8._sp, dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
+    a = A8.Wgrad8Args(G.data_ptr(), *X8._at(), dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
                       N, K, accumulate)
     _call(dev, lib.spb_gemm8_wgrad, "spb_gemm8_wgrad", code, C.byref(a))
     return dW
@@ -577,7 +584,7 @@ def act8_fwd(X, act, Y=None):
     else:
         ldy = _out(Y, (M, K), X.dtype, "Y", dev)
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, P._qp, P._sp)
+    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, *P._at())
     return Y, P
 
 
@@ -592,7 +599,7 @@ def act8_bwd(G, P, act, dX=None):
         dX, ldd = G.new_empty((M, K)), K
     else:
         ldd = _out(dX, (M, K), G.dtype, "dX", dev)
-    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, P._qp, P._sp, dX.data_ptr(), ldd, M, K)
+    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, *P._at(), dX.data_ptr(), ldd, M, K)
     return dX
 
 
