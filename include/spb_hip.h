@@ -444,9 +444,11 @@ int spb_krn_ctx_act_info(const spb_krn_ctx_t* c, int a, spb_act_info_t* out);
 /* Round 6: the expanded tensors of inverted-residual blocks 2-4 (16 -> 96 at 112x112, 24 -> 144 at 56x56) are VIRTUAL in 16-bit mode:
  * only their batch sums exist, every consumer recomputes the values (spb_dw_args_t::Xe).  spb_krn_ctx_virtual(c, a) = 1 for such a
  * tensor; spb_krn_ctx_materialize writes z of all of them into their workspace slots (z_off above) from the last forward pass's
- * state, rounded to the storage type, for tests that want to look at them.  Their g (g_off) is a real tensor. */
+ * state, rounded to the storage type, for tests that want to look at them; spb_krn_ctx_virtual_z writes one of them [B,H,W,C] in float32 (out_cap
+ * floats at `out`), the values that the kernels of the step recompute: they are never rounded there.  Their g (g_off) is a real tensor. */
 int spb_krn_ctx_virtual(const spb_krn_ctx_t* c, int a);
 int spb_krn_ctx_materialize(spb_krn_ctx_t* c, spb_stream_t stream);
+int spb_krn_ctx_virtual_z(spb_krn_ctx_t* c, int a, float* out, long long out_cap, spb_stream_t stream);
 
 /* refresh compute-dtype weight copies (W, W^T, permuted head) from the f32 parameters */
 int spb_krn_prepare_weights(spb_krn_t* m, spb_stream_t stream);

@@ -268,6 +268,7 @@ SYMBOLS = {
     "spb_hip_runtime_version": (i32, []),
     "spb_krn_ctx_virtual": (i32, [vp, i32]),
     "spb_krn_ctx_materialize": (i32, [vp, vp]),
+    "spb_krn_ctx_virtual_z": (i32, [vp, i32, vp, i64, vp]),
     "spb_det_available": (i32, []),
     "spb_det_register": (i32, [vp, i64, vp]),
     "spb_det_unregister": (i32, [vp]),

@@ -1448,6 +1448,32 @@ extern "C" int spb_krn_ctx_materialize(spb_krn_ctx_t* c, spb_stream_t stream) {
   }
   return r.err;
 }
+// The same of ONE virtual tensor as the kernels of the step see it: float32, not rounded to the storage type.
+namespace {
+__global__ __launch_bounds__(256) void virtual_z_kernel(const bf16_t* X, const bf16_t* W, float* out, long long M, int K, int N) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, m = i / N;
+  if (m >= M) return;
+  const bf16_t* x = X + m * K;
+  const bf16_t* w = W + (i - m * N) * K;
+  float v = 0.f;
+  for (int k = 0; k < K; ++k) v = fmaf(to_f<bf16_t>(x[k]), to_f<bf16_t>(w[k]), v);
+  out[i] = v;
+}
+}  // namespace
+extern "C" int spb_krn_ctx_virtual_z(spb_krn_ctx_t* c, int a, float* out, long long out_cap, spb_stream_t stream) {
+  if (!c || !out || spb_krn_ctx_virtual(c, a) != 1) return SPB_E_ARG;
+  Runner r(c, (hipStream_t)stream);
+  for (int k = 2; k <= 17; ++k) {
+    const Block& b = c->m->blk[k];
+    if (b.aE != a || !r.virt(k)) continue;
+    const long long M = r.M(a), n = M * b.E.N;
+    if (out_cap < n) return SPB_E_ARG;
+    hipLaunchKernelGGL(virtual_z_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, r.st, (const bf16_t*)r.xe_src(k).ptr,
+                       (const bf16_t*)r.wc(b.E.wc_off), out, M, b.E.K, b.E.N);
+    SPB_CHECK_LAUNCH();
+  }
+  return 0;
+}
 extern "C" int spb_krn_ctx_virtual(const spb_krn_ctx_t* c, int a) {   // 1: BatchNorm'd tensor `a` is virtual in this context (never stored)
   if (!c || a < 0 || a >= (int)c->m->acts.size()) return SPB_E_ARG;
   Runner r(const_cast<spb_krn_ctx_t*>(c), nullptr);

@@ -246,20 +246,26 @@ class KrnEngine:
                                               _stream()), "spb_krn_backward")
 
     def activations(self, batch, slot=0):
-        """{BatchNorm name: raw convolution output z of the last forward as an NCHW VIEW of the context workspace} -- what the parity
-        tests hand to the oracle to take its backward pass through this forward state (tests/test_parity_conditioned_gpu.py)"""
+        """{BatchNorm name: raw convolution output z [B,C,H,W] of the last forward} as this forward and its backward pass use it -- what the parity
+        tests hand to the oracle to take its backward pass through this forward state (tests/test_parity_conditioned_gpu.py).  Stored
+        tensors are NCHW views of the context workspace in the compute dtype.  In the 16-bit modes the expanded tensors of blocks 2-4 are
+        virtual (virtual_activations(); csrc/krn_plan.hip, Runner::virt): every kernel recomputes their values in float32 from the operand that
+        the forward pass kept, and they come as float32 tensors of their own.  (Rounded to 16 bits they were another forward state than the
+        pass's: the float64 gradients of their BatchNorms through it were off by up to 0.02 in cosine.)"""
         h, ws = self._ctx[(int(batch), int(slot))]
         dt = (torch.float16 if self.half else torch.bfloat16) if self.dtype_code == L.BF16 else torch.float32
         es = 2 if self.dtype_code == L.BF16 else 4
-        # 16-bit modes: the expanded tensors of blocks 2-4 are virtual (never stored; csrc/krn_plan.hip, Runner::virt) -- written out here,
-        # rounded to the storage type, from the operands the forward pass kept (virtual_activations() names them)
-        L.check(self.lib.spb_krn_ctx_materialize(h, _stream()), "spb_krn_ctx_materialize")
         out, ai = {}, L.ActInfo()
         for a in range(self.lib.spb_krn_num_acts(self.h)):
             L.check(self.lib.spb_krn_ctx_act_info(h, a, C.byref(ai)), "spb_krn_ctx_act_info")
+            shape = (int(batch), ai.H, ai.W, ai.C)
             n = int(batch) * ai.H * ai.W * ai.C
-            z = ws[ai.z_off: ai.z_off + n * es].view(dt).view(int(batch), ai.H, ai.W, ai.C).permute(0, 3, 1, 2)
-            out[self.bn_names[ai.bn_index][: -len(".num_batches_tracked")]] = z
+            if self.lib.spb_krn_ctx_virtual(h, a) == 1:
+                z = torch.empty(shape, dtype=torch.float32, device=ws.device)
+                L.check(self.lib.spb_krn_ctx_virtual_z(h, a, C.c_void_p(z.data_ptr()), n, _stream()), "spb_krn_ctx_virtual_z")
+            else:
+                z = ws[ai.z_off: ai.z_off + n * es].view(dt).view(shape)
+            out[self.bn_names[ai.bn_index][: -len(".num_batches_tracked")]] = z.permute(0, 3, 1, 2)
         return out
 
     def virtual_activations(self, batch, slot=0):
