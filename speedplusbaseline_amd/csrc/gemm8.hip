@@ -359,17 +359,27 @@ template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int 
 }
 
 constexpr long long ROWS_MAX = 16;
-// How a product is cut.  256 x 256 tiles do the least reading (16384 x 4096 x 4096: 211 us, 128 x 128: 261 us) but leave compute units idle below about 144 of
-// them (2816 x 4096 x 4096, 176 tiles: 49 against 54 us; 2048 x 4096 x 2048, 128 tiles: 28 against 22 us; f32 below about 192:
-// 2816 x 4096 x 1024 44 against 39 us).  128 x 128 tiles are used down to 144 of those (2352 x 1024 x 1024, 152 tiles: 8.4 us, 64 x 64: 10.1;
-// 2048 x 1024 x 1024, 128 tiles: 8.3 and 7.0).  Smaller products take 64 x 64 tiles, and where even these are fewer than 256 the reduction is split into parts of at least four steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
+// How a product is cut.  From 144 tiles of 128 x 128 on those or 256 x 256 ones are taken, whichever is estimated to end first: rounds of workgroups over the
+// 256 compute units, two of the small tile on each, times a round of KT steps.  Fitted to 130 sizes, in us: large tile 8.4 + 1.2 KT (f32 17.5 + 2.65 KT), small one
+// 3.2 + 0.75 KT (f32 8 + 1.55 KT, and 0.65 of that in a last round of one workgroup a compute unit).  Filled tiles and long reductions favour the large one, sides that
+// leave part of it empty, or start another round, the small one.  Measured, 256 against 128: 16384 x 4096 x 4096 210 / 255, 2816 x 4096 x 4096 49 / 54,
+// 37632 x 700 x 4096 101 / 111, f32 16384 x 896 x 4096 111 / 121; 150528 x 24 x 144 24 / 14, 37632 x 64 x 1024 17 / 11, 37632 x 384 x 4096 87 / 59,
+// 2048 x 4096 x 2048 27 / 19, f32 16384 x 2304 x 4096 306 / 274, f32 300 x 40000 x 1024 78 / 41.
+// f32 with a side of at most 64 takes 64 x 64 tiles, which convert nothing that is not used (150528 x 24 x 144: 20.5 us, 128: 22.9; 37632 x 64 x 1024 16.3 / 21.4; 16-bit
+// results gain nothing: 13.9 / 13.8, 11.2 / 10.7).
+// Smaller products take 64 x 64 tiles (2048 x 1024 x 1024, 128 tiles of 128: 7.0 us against 8.3), and where even these are fewer than 256 the reduction is split into parts of at least four
+// steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
 // worth that launch (3.5 us) and the partial sums' way out and back at 3.5 TB/s: 48 x 4096 x 9216 in four parts 12.4 us, in one 21.7, 300 x 512 x 4096 9.3 and
 // 11.1, but 4096 x 128 x 1024 in two parts 9.2, in one 5.1.
 struct Cut { int tile, S, steps; };
 inline Cut cut_of(bool exact, long long M, int N, int KT) {
   const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
-  if (t256 >= (exact ? 192 : 144)) return {256, 1, (KT + 3) / 4 * 4};
-  if (t128 >= 144) return {128, 1, (KT + 3) / 4 * 4};
+  if (t128 >= 144 && !(exact && (M <= 64 || N <= 64))) {
+    const long long rest = t128 % 512;
+    const double large = (double)((t256 + 255) / 256) * (exact ? 17.5 + 2.65 * KT : 8.4 + 1.2 * KT);
+    const double small = ((double)(t128 / 512) + (rest == 0 ? 0. : exact && rest <= 256 ? 0.65 : 1.)) * (exact ? 8. + 1.55 * KT : 3.2 + 0.75 * KT);
+    return {large < small ? 256 : 128, 1, (KT + 3) / 4 * 4};
+  }
   long long S = t64 >= 256 ? 1 : 256 / t64;
   const int quads = (KT + 3) / 4;
   if (S > quads) S = quads;
