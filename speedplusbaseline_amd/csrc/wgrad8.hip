@@ -363,16 +363,19 @@ template <int GR> __global__ __launch_bounds__(256) void wgrad8_join_kernel(cons
   put4(p, (f32x4_t){v.x, v.y, v.z, v.w}, K - k, accumulate);
 }
 
-struct Split { int tile, S; long long rows; };
-// 256 x 256 tiles where at least 192 of them keep the compute units busy.  Otherwise 128 x 128 or 64 x 64, the rows split for about 256 workgroups with at
+// 256 x 256 tiles where at least 192 of them keep the compute units busy and neither side is narrower than half a tile (2352 rows, 256 against 128: f16
+// 24 x 50000 116 / 93 us, f32 100 x 50000 158 / 143, bfloat16 alike; f16 200 x 50000 122 / 185; from 2^20 of them on smaller tiles
+// would be more threads than a launch holds).  Otherwise 128 x 128 or 64 x 64, the rows split for about 256 workgroups with at
 // least four stages of 64 rows each, whichever is estimated to end first: a stage of one piece takes 0.85 or 0.62 us (0.85 for 64 x 64 too where two workgroups
 // share a compute unit), two and three pieces take one and a half times and twice as long, and partial products cost a launch of 3.5 us and their way out and
 // back at 3.5 TB/s.
-// Measured in us, 128 against 64 (rows x N x K): 2352 x 1024 x 1280 26 / 34, 1024 x 1024 x 1024 19 / 13, 4096 x 1024 x 1024 30 / 42, 4096 x 512 x 512 20 / 17,
-// 300 x 1024 x 1024 10.4 / 6.6; f32 1024 x 1024 x 1024 28 / 21, 2352 x 1024 x 1280 47 / 80.
+// Measured in us, 128 against 64 (rows x N x K): 2352 x 1024 x 1280 24 / 31, 1024 x 1024 x 1024 18 / 12, 4096 x 1024 x 1024 28 / 42, 4096 x 512 x 512 18 / 16,
+// 300 x 1024 x 1024 8.9 / 6.2; f16 34 / 42, 21 / 17, 40 / 67, 21 / 20, 12.5 / 7.6; f32 37 / 76, 22 / 19, 42 / 65, 23 / 23, 14 / 8.5.
+struct Split { int tile, S; long long rows; };
 inline Split split_of(int pieces, long long M, int N, int K) {
   const long long stages = (M + 63) / 64;
-  if ((long long)((N + 255) / 256) * ((K + 255) / 256) >= 192) return {256, 1, stages * 64};
+  const long long t256 = (long long)((N + 255) / 256) * ((K + 255) / 256);
+  if (t256 >= 192 && ((N > 128 && K > 128) || t256 >= 1 << 20)) return {256, 1, stages * 64};
   Split best = {0, 1, 0};
   double least = 0;
   for (int tile = 64; tile <= 128; tile += 64) {

@@ -20,3 +20,36 @@ def test_product_of_large_and_narrow_operands(device, M, N, K, dtype):
     check_product(A, B, bias, y)
     wide = torch.full((M, N + 9), 7.0, dtype=dtype, device="cuda")
     assert torch.equal(ops.gemm8(A, B, bias=bias, dtype=dtype, Y=wide[:, 5:5 + N]), y) and (wide[:, :5] == 7).all() and (wide[:, 5 + N:] == 7).all()
+
+
+# G by LDS-DMA where N is a multiple of 8 (bfloat16), through registers otherwise: 256-wide tiles over one to six stages with a ragged last one, and sides
+# narrower than half a tile
+WGRADS = [(200, 3592, 3329), (333, 3504, 3600), (64, 3504, 3600), (130, 3590, 3400), (300, 24, 25100), (300, 50000, 24), (2352, 200, 50000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("layout", ["dense", "slab"])
+@pytest.mark.parametrize("M,N,K", WGRADS)
+def test_wgrad_of_large_and_narrow_operands(device, M, N, K, layout, dtype):
+    from speedplusbaseline_amd import ops
+    G, X8 = data(M, N, dtype, M, layout, scale=1e-3), ops.quant8(data(M, K, torch.bfloat16, N))
+    first = ops.gemm8_wgrad(G, X8)
+    check_wgrad(G, X8, first)
+    assert torch.equal(first, ops.gemm8_wgrad(G, X8))
+    wide = torch.randn(N, K + 5, device="cuda")
+    before = wide.clone()
+    out = ops.gemm8_wgrad(G, X8, dW=wide[:, 2:2 + K])
+    check_wgrad(G, X8, out, before[:, 2:2 + K].double())
+    assert torch.equal(wide[:, :2], before[:, :2]) and torch.equal(wide[:, 2 + K:], before[:, 2 + K:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_wgrad_rows_and_columns_behind_the_matrix_do_not_count(device, dtype):
+    """ragged ends in a matrix of NaN: rows behind the last one, columns beside G"""
+    from speedplusbaseline_amd import ops
+    M, N, K = 200, 3592, 3400
+    wide = torch.full((M + 60, N + 8), float("nan"), dtype=dtype, device="cuda")
+    wide[:M, :N] = data(M, N, dtype, 3, scale=1e-3)
+    X8 = ops.quant8(data(M, K, torch.bfloat16, 4))
+    dw = ops.gemm8_wgrad(wide[:M, :N], X8)
+    assert dw.isfinite().all() and torch.equal(dw, ops.gemm8_wgrad(wide[:M, :N].contiguous(), X8))
