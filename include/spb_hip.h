@@ -705,7 +705,7 @@ int spb_preproc_batch(const spb_preproc_args_t* a, spb_stream_t stream);
 /* ---- layer norm (csrc/layernorm.hip): y = (x - mean) * rstd * gamma + beta over the last axis of [M, C] rows ---------------------------
  * mean and rstd = 1 / sqrt(var + eps) (biased variance) are per row, f32, written by the forward and read by the backward.  dtype names X, G
  * and Y; gamma, beta and their gradients are f32; gamma == NULL: 1, beta == NULL: 0.  Rows may have any stride (elements), columns are
- * contiguous.  C >= 1; M == 0 launches nothing except a requested write of zero gradients. */
+ * contiguous.  1 <= C <= 2^30, with dgamma or dbeta C <= 2^27 - 64; M == 0 launches nothing except a requested write of zero gradients. */
 typedef struct spb_layernorm_args {
   const void* X;       /* [M,C], row stride ldx */
   const void* G;       /* backward: dL/dy [M,C], row stride ldg */
@@ -736,7 +736,8 @@ long long spb_layernorm_bwd_floats(long long M, int C);
  * An element stands for code * 2^e.  e is the smallest integer with max |x| <= 448 * 2^e over the block's FINITE elements, kept in [-110, 120]
  * (0 for a block without finite nonzero elements); x * 2^-e is exact and is rounded to the nearest code, ties to even.  Infinities and NaN become NaN.
  * Every value is exact in bfloat16 and float32 (magnitudes that would round up to 2^128 take the code below).
- * Code buffers are 16-byte aligned, scale buffers 4-byte aligned. */
+ * Code buffers are 16-byte aligned, scale buffers 4-byte aligned.  By rows: M * ceil(K / 8) < 2^32 - 16 vectors (packing alone: M * ceil(K / 128) blocks);
+ * weights: fewer than 2^24 blocks of 128 x 128. */
 int spb_pack8_rows(int dtype, const void* X, long long ldx, long long M, int K, unsigned char* codes, unsigned char* scales, spb_stream_t stream);
 /* 128 x 128 blocks of W [N,K]; codesT / scalesT (both or neither NULL) receive the packed transpose [K,N]: the same values, the operand of the
  * input gradient */

@@ -341,16 +341,17 @@ template <typename TO, int GR> __global__ __launch_bounds__(256) void gemm8_join
 
 // no reduction (K == 0): the bias alone
 template <typename TO> __global__ __launch_bounds__(256) void gemm8_bias_kernel(const Gemm8Args g) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long m = i / g.N;
-  const int n = (int)(i - m * g.N);
-  if (m < g.M) reinterpret_cast<TO*>(g.Y)[m * g.ldy + n] = from_f<TO>(g.bias ? g.bias[n] : 0.f);
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < g.M * g.N; i += (long long)gridDim.x * 256) {
+    const long long m = i / g.N;
+    const int n = (int)(i - m * g.N);
+    reinterpret_cast<TO*>(g.Y)[m * g.ldy + n] = from_f<TO>(g.bias ? g.bias[n] : 0.f);
+  }
 }
 
 template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int run(const Gemm8Args& g, int S, hipStream_t s) {
   constexpr int LDS = NST * (BM + BN) * 132;
   const long long wgs = (g.M + BM - 1) / BM * ((g.N + BN - 1) / BN) * S;
-  if (wgs > 0x7fffffffll) return SPB_E_SHAPE;
+  if (!p8_fits(wgs, WM * WN * 64)) return SPB_E_SHAPE;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm8_kernel<BM, BN, WM, WN, NST, EXACT, TO>), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (e != hipSuccess) return (int)e;
   hipLaunchKernelGGL((gemm8_kernel<BM, BN, WM, WN, NST, EXACT, TO>), dim3((unsigned)wgs), dim3(WM * WN * 64), LDS, s, g);
@@ -358,7 +359,8 @@ template <int BM, int BN, int WM, int WN, int NST, bool EXACT, typename TO> int 
   return 0;
 }
 
-constexpr long long ROWS_MAX = 16;
+// the rows kernel: few rows, and columns for which a launch has threads
+inline bool by_rows(long long M, int N) { return M <= 16 && p8_fits((N + 15) / 16, SKW * 64); }
 // How a product is cut.  From 144 tiles of 128 x 128 on those or 256 x 256 ones are taken, whichever is estimated to end first: rounds of workgroups over the
 // 256 compute units, two of the small tile on each, times a round of KT steps.  Fitted to 130 sizes, in us: large tile 8.4 + 1.2 KT (f32 17.5 + 2.65 KT), small one
 // 3.2 + 0.75 KT (f32 8 + 1.55 KT, and 0.65 of that in a last round of one workgroup a compute unit).  Filled tiles and long reductions favour the large one, sides that
@@ -374,6 +376,7 @@ constexpr long long ROWS_MAX = 16;
 struct Cut { int tile, S, steps; };
 inline Cut cut_of(bool exact, long long M, int N, int KT) {
   const long long t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128), t64 = (M + 63) / 64 * ((N + 63) / 64);
+  if (t256 >= 1 << 20) return {256, 1, (KT + 3) / 4 * 4};         // smaller tiles would be more threads than a launch holds
   if (t128 >= 144 && !(exact && (M <= 64 || N <= 64))) {
     const long long rest = t128 % 512;
     const double large = (double)((t256 + 255) / 256) * (exact ? 17.5 + 2.65 * KT : 8.4 + 1.2 * KT);
@@ -389,7 +392,7 @@ inline Cut cut_of(bool exact, long long M, int N, int KT) {
   return {64, (int)S, per * 4};
 }
 template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hipStream_t s) {
-  if (g.M <= ROWS_MAX) {
+  if (by_rows(g.M, g.N)) {
     hipLaunchKernelGGL((gemm8_rows_kernel<TO>), dim3((unsigned)((g.N + 15) / 16)), dim3(SKW * 64), 0, s, g);
     SPB_CHECK_LAUNCH();
     return 0;
@@ -422,7 +425,7 @@ template <bool EXACT, typename TO> int product(const Gemm8Args& g, void* ws, hip
 
 extern "C" long long spb_gemm8_bytes(int dtype, long long M, int N, int K) {
   if ((dtype != SPB_F32 && dtype != SPB_BF16) || M < 0 || N < 0 || N > P8_SIDE_MAX || K < 0 || K > P8_DEPTH_MAX) return SPB_E_SHAPE;
-  if (M <= ROWS_MAX || N == 0 || K == 0) return 0;
+  if (M == 0 || N == 0 || K == 0 || by_rows(M, N)) return 0;
   const Cut c = cut_of(dtype == SPB_F32, M, N, (K + 127) / 128);
   return c.S > 1 ? (long long)c.S * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
@@ -435,8 +438,7 @@ extern "C" int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stre
   hipStream_t s = (hipStream_t)stream;
   Gemm8Args g = {a->A, a->As, a->B, a->Bs, a->bias, a->Y, a->M, a->ldy, 0, a->N, p8_cols(a->K), p8_scales(a->K), a->b_block_rows == 128 ? 7 : 0, 0};
   if (a->K == 0) {
-    const long long blocks = (a->M * a->N + 255) / 256;
-    if (blocks > 0x7fffffffll) return SPB_E_SHAPE;
+    const long long all = (a->M * a->N + 255) / 256, blocks = all < 1 << 20 ? all : 1 << 20;
     if (dtype == SPB_F32) hipLaunchKernelGGL((gemm8_bias_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, s, g);
     else hipLaunchKernelGGL((gemm8_bias_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, s, g);
     SPB_CHECK_LAUNCH();

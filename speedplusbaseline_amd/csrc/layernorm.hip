@@ -17,6 +17,8 @@
 namespace {
 
 constexpr int LN_REG_MAX = 8192;      // longest row held in registers
+constexpr int LN_COLS_MAX = 1 << 30;  // column counters of long rows step past the end
+constexpr int LN_SUMS_MAX = (1 << 27) - 64;   // longest row with parameter gradients: the launch that joins their partial rows has 16 threads for each of 2 C sums
 constexpr int LN_FWD_WGS = 2048;      // workgroups that walk the rows: eight of 256 threads on each of the 256 compute units
 constexpr int LN_BWD_WGS = 512;       // backward: each stores one partial row of 2 C floats, so fewer of them
 
@@ -385,7 +387,8 @@ template <typename T> int run_bwd(const spb_layernorm_args_t& a, bool sums, hipS
 
 int check_args(int dtype, const spb_layernorm_args_t* a, bool bwd) {
   if (dtype != SPB_F32 && dtype != SPB_BF16) return SPB_E_ARG;
-  if (!a || a->C < 1 || a->M < 0) return a ? SPB_E_SHAPE : SPB_E_ARG;
+  if (!a || a->C < 1 || a->C > LN_COLS_MAX || a->M < 0) return a ? SPB_E_SHAPE : SPB_E_ARG;
+  if (bwd && (a->dgamma || a->dbeta) && a->C > LN_SUMS_MAX) return SPB_E_SHAPE;
   if (a->M == 0) return 0;
   if (!a->X || !a->Y || !a->mean || !a->rstd || (bwd && !a->G)) return SPB_E_ARG;
   if (a->ldx < 0 || a->ldy < (a->M > 1 ? a->C : 0) || (bwd && a->ldg < 0)) return SPB_E_SHAPE;
@@ -405,7 +408,7 @@ extern "C" int spb_layernorm_fwd(int dtype, const spb_layernorm_args_t* a, spb_s
 }
 
 extern "C" long long spb_layernorm_bwd_floats(long long M, int C) {
-  if (M < 0 || C < 1) return SPB_E_SHAPE;
+  if (M < 0 || C < 1 || C > LN_SUMS_MAX) return SPB_E_SHAPE;
   return 2ll * C * ln_bwd_parts(M, C);
 }
 

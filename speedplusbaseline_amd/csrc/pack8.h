@@ -12,6 +12,9 @@
 static inline int p8_cols(int K) { return (K + 127) / 128 * 128; }          // Kp: bytes of a row of codes
 static inline int p8_scales(int K) { return ((K + 127) / 128 + 3) / 4 * 4; } // Sp: bytes of a row of scales
 
+#define P8_THREADS 0xffffffffll        // most threads that a launch holds
+static inline bool p8_fits(long long wgs, int threads) { return wgs <= 0x7fffffffll && wgs * threads <= P8_THREADS; }
+
 // exponent of a block from its largest finite magnitude: top = m 2^k with 1 <= m < 2 and 448 = 1.75 * 2^8, so e = k - 8, one more if m > 1.75
 __device__ __forceinline__ int p8_exponent(float top) {
   const unsigned u = __float_as_uint(top);

@@ -236,16 +236,30 @@ inline bool bad_dtype(int d) { return d != SPB_F32 && d != SPB_BF16; }
     SPB_CHECK_LAUNCH();                                                                                                                     \
   } while (0)
 
+// as many rows a launch as it has threads for (16 a block; 8 elements each)
 template <int ACT> int pack_rows(int dtype, RowArgs a, long long M, hipStream_t s) {
   if (M * a.KB > 0xfffffff0ll) return SPB_E_SHAPE;
-  a.blocks = (unsigned)(M * a.KB);
-  P8_LAUNCH(pack8_rows_kernel, dim3(a.blocks / 16 + (a.blocks % 16 ? 1 : 0)), ACT);
+  const long long most = (P8_THREADS / 256 * 16) / a.KB, es = dtype == SPB_F32 ? 4 : 2;
+  for (; M > 0; M -= most) {
+    a.blocks = (unsigned)((M < most ? M : most) * a.KB);
+    P8_LAUNCH(pack8_rows_kernel, dim3(a.blocks / 16 + (a.blocks % 16 ? 1 : 0)), ACT);
+    a.X = (const char*)a.X + most * a.ldx * es; a.Q += most * a.Kp; a.S += most * a.Sp;
+    if (ACT != 0) a.Y = (char*)a.Y + most * a.ldy * es;
+  }
   return 0;
 }
 template <int ACT> int unpack(int dtype, UnpackArgs a, long long M, hipStream_t s) {
   if (M * a.V > 0xfffffff0ll) return SPB_E_SHAPE;
-  a.vecs = (unsigned)(M * a.V);
-  P8_LAUNCH(unpack8_kernel, dim3(a.vecs / 256 + (a.vecs % 256 ? 1 : 0)), ACT);
+  long long most = (P8_THREADS / 256 * 256) / a.V;
+  const long long es = dtype == SPB_F32 ? 4 : 2;
+  if (most < M && a.shift) most = most >> 7 << 7;       // whole blocks of rows
+  if (most == 0) return SPB_E_SHAPE;
+  for (; M > 0; M -= most) {
+    a.vecs = (unsigned)((M < most ? M : most) * a.V);
+    P8_LAUNCH(unpack8_kernel, dim3(a.vecs / 256 + (a.vecs % 256 ? 1 : 0)), ACT);
+    a.Q += most * a.Kp; a.S += (most >> a.shift) * a.Sp; a.Y = (char*)a.Y + most * a.ldy * es;
+    if (ACT != 0) a.G = (const char*)a.G + most * a.ldg * es;
+  }
   return 0;
 }
 
@@ -266,7 +280,7 @@ extern "C" int spb_pack8_weight(int dtype, const void* W, long long ldw, int N, 
   if (N == 0 || K == 0) return 0;
   if (!W || bad_codes(codes, scales) || (codesT != nullptr) != (scalesT != nullptr) || (codesT && bad_codes(codesT, scalesT))) return SPB_E_ARG;
   const WeightArgs a = {W, codes, scales, codesT, scalesT, ldw, N, K, (N + 127) / 128, (K + 127) / 128, p8_cols(K), p8_scales(K), p8_cols(N), p8_scales(N)};
-  if ((long long)a.NB * a.KB > 0x7fffffffll) return SPB_E_SHAPE;
+  if (!p8_fits((long long)a.NB * a.KB, 256)) return SPB_E_SHAPE;
   hipStream_t s = (hipStream_t)stream;
   P8_LAUNCH(pack8_weight_kernel, dim3((unsigned)(a.NB * a.KB)));
   return 0;

@@ -414,7 +414,7 @@ template <typename T, int P, bool GDMA, int MODE, int NST, int WN, int WK, int T
 }
 template <typename T, int P, bool GDMA, int MODE> int run(Wgrad8Args g, const Split& sp, hipStream_t s) {
   g.NT = (g.N + sp.tile - 1) / sp.tile; g.KT = (g.K + sp.tile - 1) / sp.tile;
-  if ((long long)g.NT * g.KT * sp.S > 0x7fffffffll) return SPB_E_SHAPE;
+  if (!p8_fits((long long)g.NT * g.KT * sp.S, 512)) return SPB_E_SHAPE;
   if (sp.tile == 256) return launch<T, P, GDMA, MODE, 2, 2, 4, 8, 4>(g, sp.S, s);
   if (sp.tile == 64) return launch<T, P, GDMA, MODE, 4, 2, 2, 2, 2>(g, sp.S, s);
   return launch<T, P, GDMA, MODE, 4, 2, 4, 4, 2>(g, sp.S, s);
@@ -424,9 +424,10 @@ template <typename T, int P> int run_regs(const Wgrad8Args& g, const Split& sp, 
   return mode == 0 ? run<T, P, false, 0>(g, sp, s) : (mode == 1 ? run<T, P, false, 1>(g, sp, s) : run<T, P, false, 2>(g, sp, s));
 }
 __global__ __launch_bounds__(256) void wgrad8_zero_kernel(float* dW, long long ldw, int N, int K) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long n = i / K;
-  if (n < N) dW[n * ldw + (i - n * K)] = 0.f;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)N * K; i += (long long)gridDim.x * 256) {
+    const long long n = i / K;
+    dW[n * ldw + (i - n * K)] = 0.f;
+  }
 }
 
 }  // namespace
@@ -444,10 +445,9 @@ extern "C" int spb_gemm8_wgrad(int dtype, const spb_wgrad8_args_t* a, spb_stream
   if (a->N == 0 || a->K == 0) return 0;
   if (!a->dW) return SPB_E_ARG;
   hipStream_t s = (hipStream_t)stream;
-  const long long blocks1 = ((long long)a->N * a->K + 255) / 256;
-  if (blocks1 > 0x7fffffffll) return SPB_E_SHAPE;
   if (a->M == 0) {
-    if (!a->accumulate) hipLaunchKernelGGL(wgrad8_zero_kernel, dim3((unsigned)blocks1), dim3(256), 0, s, a->dW, a->ldw, a->N, a->K);
+    const long long all = ((long long)a->N * a->K + 255) / 256;
+    if (!a->accumulate) hipLaunchKernelGGL(wgrad8_zero_kernel, dim3((unsigned)(all < 1 << 20 ? all : 1 << 20)), dim3(256), 0, s, a->dW, a->ldw, a->N, a->K);
     SPB_CHECK_LAUNCH();
     return 0;
   }
