@@ -775,7 +775,8 @@ typedef struct spb_gemm8_args {
 int spb_gemm8(int dtype, const spb_gemm8_args_t* a, spb_stream_t stream);
 long long spb_gemm8_bytes(int dtype, long long M, int N, int K);
 /* dW[n,k] (+)= sum_m G[m,n] * X[m,k] with X packed by rows (a layer's 8-bit checkpoint of its input).  G is NOT rounded: a 16-bit or f32 gradient is
- * split into one (bfloat16), two (half) or three (float32) bfloat16 pieces whose sum is exact, and every product is exact.  dW f32, row stride ldw. */
+ * split into one (bfloat16), two (half) or three (float32) bfloat16 pieces whose sum is exact, and every product is exact.
+ * Infinities and NaN in G spread as in the sum of products itself.  dW f32, row stride ldw. */
 typedef struct spb_wgrad8_args {
   const void* G;           /* [M,N], row stride ldg */
   const unsigned char* X;  /* [M][Kp] codes */

@@ -30,9 +30,11 @@ struct Wgrad8Args {
   int N, K, Kp, Sp, NT, KT, accumulate;
 };
 
-// bfloat16 pieces of 8 gradients, piece p of all of them in out[p]: the upper half of the bits, then the same of what is left.  The differences are exact; a
-// gradient that is not finite leaves NaN in the second piece, and its row of dW is NaN.
+// bfloat16 pieces of 8 gradients, piece p of all of them in out[p]: the upper half of the bits, then the same of what is left.  The differences are exact.  What is
+// subtracted is kept finite: every piece of an infinity is one (inf - inf would make its row of dW NaN where bfloat16 gradients give infinities), and a NaN
+// stays one in the second piece whatever its bits.  It costs an instruction an element: f16 16384 x 4096 x 4096 815 -> 823 us, f32 1183 -> 1198.
 template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 out[P]) {
+  constexpr float TOP = 3.4028234e38f;
   float r[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = v[i];
@@ -44,7 +46,7 @@ template <int P> __device__ __forceinline__ void split8(const float v[8], uint4 
     out[p] = make_uint4(__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u),
                         __builtin_amdgcn_perm(u[5], u[4], 0x07060302u), __builtin_amdgcn_perm(u[7], u[6], 0x07060302u));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] -= __uint_as_float(u[i] & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) r[i] -= __builtin_amdgcn_fmed3f(__uint_as_float(u[i] & 0xffff0000u), -TOP, TOP);
   }
 }
 // Four neighbouring values of a row (`left` of them inside it), added to what is there or not, at any alignment (element by element: 71 x 3494 x 958

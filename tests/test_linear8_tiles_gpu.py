@@ -53,3 +53,18 @@ def test_wgrad_rows_and_columns_behind_the_matrix_do_not_count(device, dtype):
     X8 = ops.quant8(data(M, K, torch.bfloat16, 4))
     dw = ops.gemm8_wgrad(wide[:M, :N], X8)
     assert dw.isfinite().all() and torch.equal(dw, ops.gemm8_wgrad(wide[:M, :N].contiguous(), X8))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K", [(3, 8, 130), (70, 40, 300), (2400, 1024, 1200), (70, 3504, 3600), (70, 3501, 3600)])
+def test_wgrad_of_infinite_gradients(device, M, N, K, dtype):
+    """infinities of the same places and signs as in the sum of products itself, whatever the type; NaN where they meet a zero or each other"""
+    from speedplusbaseline_amd import ops
+    G, x = data(M, N, dtype, M, scale=1e-3), data(M, K, torch.bfloat16, N)
+    G[1, 2], G[2, 5], G[0, 5], G[2, 7] = float("inf"), -float("inf"), float("inf"), float("nan")
+    X8 = ops.quant8(x)
+    dw = ops.gemm8_wgrad(G, X8)
+    want = G.double().t() @ ops.dequant8(X8, torch.float32).double()
+    assert want[2].isinf().any() and want[5].isnan().any() and want[7].isnan().all()
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(dw), f(want)), f.__name__
