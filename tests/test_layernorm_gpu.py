@@ -221,7 +221,7 @@ def test_backward_empty_and_same_bits_twice(device):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
-def test_rows_behind_two_to_the_32(device):
+def test_longest_register_rows_behind_two_to_the_32(device):
     """more than 2^32 bytes in front of the last rows"""
     from speedplusbaseline_amd import ops
     M, C = 300000, 8192                                     # 4.9 GB of bfloat16
