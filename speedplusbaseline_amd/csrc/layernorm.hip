@@ -283,17 +283,21 @@ __global__ __launch_bounds__(256) void ln_bwd_long(const spb_layernorm_args_t a)
   }
 }
 // partial rows of dgamma / dbeta for long rows: a thread a column, blockIdx.y a range of rows.  It runs BEFORE ln_bwd_long, whose output may
-// overwrite g.
+// overwrite g.  Rows are added in blocks of 64, whose sums are added up: a single chain would collect a rounding for each of the range's rows.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_cols(const spb_layernorm_args_t a, long long rows) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   const long long m0 = (long long)blockIdx.y * rows, m1 = m0 + rows < a.M ? m0 + rows : a.M;
   if (c >= a.C) return;
   float dg = 0.f, db = 0.f;
-  for (long long m = m0; m < m1; ++m) {
-    const float g = to_f<T>(reinterpret_cast<const T*>(a.G)[m * a.ldg + c]);
-    dg += g * (to_f<T>(reinterpret_cast<const T*>(a.X)[m * a.ldx + c]) - a.mean[m]) * a.rstd[m];
-    db += g;
+  for (long long b = m0; b < m1; b += 64) {
+    float pg = 0.f, pb = 0.f;
+    for (long long m = b, e = b + 64 < m1 ? b + 64 : m1; m < e; ++m) {
+      const float g = to_f<T>(reinterpret_cast<const T*>(a.G)[m * a.ldg + c]);
+      pg += g * (to_f<T>(reinterpret_cast<const T*>(a.X)[m * a.ldx + c]) - a.mean[m]) * a.rstd[m];
+      pb += g;
+    }
+    dg += pg; db += pb;
   }
   float* out = a.part + (size_t)blockIdx.y * 2 * a.C;
   out[c] = dg; out[a.C + c] = db;
