@@ -396,6 +396,7 @@ int check_args(int dtype, const spb_layernorm_args_t* a, bool bwd) {
   if (a->M == 0) return 0;
   if (!a->X || !a->Y || !a->mean || !a->rstd || (bwd && !a->G)) return SPB_E_ARG;
   if (a->ldx < 0 || a->ldy < (a->M > 1 ? a->C : 0) || (bwd && a->ldg < 0)) return SPB_E_SHAPE;
+  if (bwd && a->dgamma && a->dgamma == a->dbeta) return SPB_E_ARG;      // two sums into one buffer
   return 0;
 }
 
