@@ -436,73 +436,94 @@ def layernorm_bwd(G, X, mean, rstd, gamma=None, dgamma=None, dbeta=None, dX=None
 
 class Packed8:
     """A matrix in e4m3 codes with one power-of-two scale for each block of 128 (include/spb_hip.h "8-bit packing"): codes uint8 [rows, K rounded up to
-    128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight).  Copies (copy, pickle, torch.save) hold their own tensors: device
-    and addresses are those of `_own` at the time of a call, never kept beside it."""
-    __slots__ = ("K", "block_rows", "shape", "_rows", "_own")
+    128], scales uint8 (exponent + 127); block_rows 1 (quant8) or 128 (quant8_weight).
+    A matrix made by `empty` owns one buffer, which nobody else can move, and keeps its device and addresses (1 us of a call's 7); copies (copy, pickle, torch.save) are
+    built anew from the copied tensors.  One made of a caller's tensors asks them at every call."""
+    __slots__ = ("K", "block_rows", "shape", "_rows", "_own", "_dev", "_qp", "_sp")
 
     def __init__(self, codes, scales, K, block_rows):
-        kb = (K + 127) // 128
         if block_rows not in (1, 128) or K < 0 or codes.dim() != 2:
             raise RuntimeError("Packed8: block_rows must be 1 or 128 and the codes a matrix")
         rows = codes.shape[0]
-        for t, shape in ((codes, (rows, kb * 128)), (scales, ((rows + block_rows - 1) // block_rows, (kb + 3) // 4 * 4))):
-            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
-                raise RuntimeError("Packed8: codes and scales do not fit a packed [%d, %d] matrix" % (rows, K))
         self.K, self.block_rows, self.shape, self._rows = K, block_rows, (rows, K), rows
-        self._own = codes, scales
+        self._own, self._dev = (codes, scales), None
+        self._check()
+
+    def _check(self):
+        """a caller's tensors: also at every call, since they may have been given other storage"""
+        codes, scales = self._own
+        kb, rows = (self.K + 127) // 128, self._rows
+        for t, shape in ((codes, (rows, kb * 128)), (scales, ((rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != codes.device:
+                raise RuntimeError("Packed8: codes and scales do not fit a packed [%d, %d] matrix" % (rows, self.K))
 
     @staticmethod
     def empty(rows, K, block_rows, device):
         """uninitialised; codes and scales share one allocation"""
         kb = (K + 127) // 128
         buf = torch.empty(rows * kb * 128 + (rows + block_rows - 1) // block_rows * ((kb + 3) // 4 * 4), dtype=torch.uint8, device=device)
+        return Packed8._around(buf, rows, K, block_rows)
+
+    @staticmethod
+    def _around(buf, rows, K, block_rows):
         self = Packed8.__new__(Packed8)
         self.K, self.block_rows, self.shape, self._rows = K, block_rows, (rows, K), rows
-        self._own = (buf,)
+        self._own, self._dev, self._qp = buf, buf.get_device(), buf.data_ptr()
+        self._sp = self._qp + rows * ((K + 127) // 128) * 128
         return self
+
+    def __reduce__(self):
+        if self._dev is None:
+            return Packed8, (*self._own, self.K, self.block_rows)
+        return Packed8._around, (self._own, self._rows, self.K, self.block_rows)
 
     @property
     def device(self):
-        return self._own[0].device
+        return (self._own[0] if self._dev is None else self._own).device
 
     @property
     def codes(self):
-        if len(self._own) == 2:
+        if self._dev is None:
             return self._own[0]
         kp = (self.K + 127) // 128 * 128
-        return self._own[0][:self._rows * kp].view(self._rows, kp)
+        return self._own[:self._rows * kp].view(self._rows, kp)
 
     @property
     def scales(self):
-        if len(self._own) == 2:
+        if self._dev is None:
             return self._own[1]
         kb = (self.K + 127) // 128
-        return self._own[0][self._rows * kb * 128:].view((self._rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4)
+        return self._own[self._rows * kb * 128:].view((self._rows + self.block_rows - 1) // self.block_rows, (kb + 3) // 4 * 4)
 
     def _at(self):
         """addresses of the codes and the scales"""
-        own = self._own
-        q = own[0].data_ptr()
-        return q, (own[1].data_ptr() if len(own) == 2 else q + self._rows * ((self.K + 127) // 128) * 128)
+        if self._dev is None:
+            return self._own[0].data_ptr(), self._own[1].data_ptr()
+        return self._qp, self._sp
 
 
 def _packed(P, name, dev=None, block_rows=None):
-    """checks a Packed8 operand; returns its device"""
+    """checks a Packed8 operand; returns its device and the addresses of its codes and scales"""
     if not isinstance(P, Packed8):
         raise RuntimeError("%s must be a Packed8 (quant8 / quant8_weight), got %s" % (name, type(P).__name__))
     if block_rows is not None and P.block_rows != block_rows:
         raise RuntimeError("%s must be packed in blocks of %d x 128" % (name, block_rows))
-    on = P._own[0].get_device()
+    on = P._dev
+    if on is None:
+        P._check()
+        on = P._own[0].get_device()
     if on < 0 or (dev is not None and on != dev):
         raise RuntimeError("%s is on %s, expected %s" % (name, P.device, "a GPU" if dev is None else "device %d" % dev))
-    return on
+    if P._dev is None:
+        return on, *P._at()
+    return on, P._qp, P._sp
 
 
 def quant8(X):
     """X [M, K] packed in blocks of 1 x 128: operand of gemm8 and checkpoint for gemm8_wgrad"""
     dev, M, K, ldx, code = _mat(X, "X")
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, *P._at())
+    _call(dev, _lib8(X.dtype).spb_pack8_rows, "spb_pack8_rows", code, X.data_ptr(), ldx, M, K, P._qp, P._sp)
     return P
 
 
@@ -511,26 +532,26 @@ def quant8_weight(W, transpose=True):
     dev, N, K, ldw, code = _mat(W, "W")
     P = Packed8.empty(N, K, 128, W.device)
     T = Packed8.empty(K, N, 128, W.device) if transpose else None
-    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, *P._at(),
-          *(T._at() if transpose else (None, None)))
+    _call(dev, _lib8(W.dtype).spb_pack8_weight, "spb_pack8_weight", code, W.data_ptr(), ldw, N, K, P._qp, P._sp,
+          T._qp if transpose else None, T._sp if transpose else None)
     return P, T
 
 
 def dequant8(P, dtype=torch.bfloat16, Y=None):
     """the values of a Packed8 (exact in bfloat16 and float32)"""
-    dev = _packed(P, "P")
+    dev, qp, sp = _packed(P, "P")
     if Y is None:
         Y = torch.empty(P.shape, dtype=dtype, device=P.device)
     ldy = _out(Y, P.shape, dtype, "Y", dev)
-    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], *P._at(), P.block_rows, P._rows, P.K, Y.data_ptr(), ldy)
+    _call(dev, _lib8(dtype).spb_unpack8, "spb_unpack8", _DT[dtype], qp, sp, P.block_rows, P._rows, P.K, Y.data_ptr(), ldy)
     return Y
 
 
 def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
     """Y [M, N] = A [M, K] (quant8) times the transpose of B [N, K] (quant8_weight or quant8) + bias (float32 [N]).  dtype float32: the products run
     through the bfloat16 matrix instructions, where they are exact; 16-bit types: through the 8-bit ones."""
-    dev = _packed(A, "A", None, 1)
-    _packed(B, "B", dev)
+    dev, aq, a_s = _packed(A, "A", None, 1)
+    _, bq, bs = _packed(B, "B", dev)
     if A.K != B.K:
         raise RuntimeError("gemm8: A has %d columns, B has %d" % (A.K, B.K))
     M, N, K = A._rows, B._rows, A.K
@@ -543,7 +564,7 @@ def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
     lib, code = _lib8(dtype), _DT[dtype]
     need = lib.spb_gemm8_bytes(code, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=A.device) if need > 0 else None
-    a = A8.Gemm8Args(*A._at(), *B._at(), _vec(bias, N, "bias", dev), Y.data_ptr(),
+    a = A8.Gemm8Args(aq, a_s, bq, bs, _vec(bias, N, "bias", dev), Y.data_ptr(),
                      None if ws is None else ws.data_ptr(), need, M, ldy, N, K, B.block_rows)
     _call(dev, lib.spb_gemm8, "spb_gemm8", code, C.byref(a))
     return Y
@@ -552,7 +573,7 @@ def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
 def gemm8_wgrad(G, X8, dW=None):
     """dW [N, K] (float32) = transpose of G [M, N] times the checkpoint X8 (quant8 of the layer's input [M, K]); dW given: accumulated into"""
     dev, M, N, ldg, code = _mat(G, "G")
-    _packed(X8, "X8", dev, 1)
+    _, xq, xs = _packed(X8, "X8", dev, 1)
     K = X8.K
     if X8._rows != M:
         raise RuntimeError("gemm8_wgrad: G has %d rows, X8 has %d" % (M, X8._rows))
@@ -564,7 +585,7 @@ def gemm8_wgrad(G, X8, dW=None):
     lib = _lib8(G.dtype)
     need = lib.spb_gemm8_wgrad_bytes(code, M, N, K)
     ws = torch.empty(need, dtype=torch.uint8, device=G.device) if need > 0 else None
-    a = A8.Wgrad8Args(G.data_ptr(), *X8._at(), dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
+    a = A8.Wgrad8Args(G.data_ptr(), xq, xs, dW.data_ptr(), None if ws is None else ws.data_ptr(), need, M, ldg, ldw,
                       N, K, accumulate)
     _call(dev, lib.spb_gemm8_wgrad, "spb_gemm8_wgrad", code, C.byref(a))
     return dW
@@ -584,7 +605,7 @@ def act8_fwd(X, act, Y=None):
     else:
         ldy = _out(Y, (M, K), X.dtype, "Y", dev)
     P = Packed8.empty(M, K, 1, X.device)
-    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, *P._at())
+    _call(dev, _lib8(X.dtype).spb_act8_fwd, "spb_act8_fwd", code, act, X.data_ptr(), ldx, Y.data_ptr(), ldy, M, K, P._qp, P._sp)
     return Y, P
 
 
@@ -592,14 +613,14 @@ def act8_bwd(G, P, act, dX=None):
     """dX = G * act'(value of the checkpoint P).  dX: optional output of G's type, may be G itself."""
     _act8(act)
     dev, M, K, ldg, code = _mat(G, "G")
-    _packed(P, "P", dev, 1)
+    _, qp, sp = _packed(P, "P", dev, 1)
     if P._rows != M or P.K != K:
         raise RuntimeError("act8_bwd: G is %s, the checkpoint %s" % ((M, K), P.shape))
     if dX is None:
         dX, ldd = G.new_empty((M, K)), K
     else:
         ldd = _out(dX, (M, K), G.dtype, "dX", dev)
-    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, *P._at(), dX.data_ptr(), ldd, M, K)
+    _call(dev, _lib8(G.dtype).spb_act8_bwd, "spb_act8_bwd", code, act, G.data_ptr(), ldg, qp, sp, dX.data_ptr(), ldd, M, K)
     return dX
 
 

@@ -41,6 +41,32 @@ def test_copies_have_their_own_addresses(how, separate):
     assert P.codes.any()
 
 
+def test_a_callers_tensors_with_other_storage():
+    """what Module.to does to a parameter: the tensor object stays, its storage is another one"""
+    P = one(5, 300, 1, "cpu", True)
+    codes, scales = P._own
+    codes.data = codes.data.clone()
+    assert P._at() == (codes.data_ptr(), scales.data_ptr())
+    ops.Packed8._check(P)
+    for wrong in (torch.zeros(4, 384, dtype=torch.uint8), torch.zeros(5, 384, dtype=torch.int8), torch.zeros(384, 5, dtype=torch.uint8).t()):
+        codes.data = wrong
+        with pytest.raises(RuntimeError):
+            P._check()
+
+
+@pytest.mark.gpu
+def test_products_after_other_storage(device):
+    A, B = one(37, 300, 1, "cuda", True), one(130, 300, 128, "cuda", False)
+    want = ops.gemm8(A, B)
+    codes = A._own[0]
+    old, codes.data = codes.data, codes.data.clone()
+    old.zero_()
+    assert torch.equal(ops.gemm8(A, B), want)
+    codes.data = codes.data.cpu()
+    with pytest.raises(RuntimeError):
+        ops.gemm8(A, B)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("separate", [False, True])
 @pytest.mark.parametrize("how", COPIES, ids=["deepcopy", "pickle", "save"])
