@@ -294,9 +294,9 @@ int spb_grad_sqnorm_partials(const float* grads, long long n, float* partials_ou
  * backward passes of a DANN step accumulate into one gradient, dann.py:95); n elements, n % 4 == 0 for the add */
 int spb_arena_zero(float* arena, long long n, spb_stream_t stream);
 int spb_arena_add(float* dst, const float* src, long long n, spb_stream_t stream);
-/* A HIP stream at the device's highest (level < 0), default (0) or lowest (level > 0) dispatch priority.  The SPN step runs
- * its 0.8 ms HBM-bound parameter update on a lowest-priority stream beside the trunk's backward: the dispatcher then fills
- * the launch stream's kernels first and the update takes what they leave (host side: nets/spn.py loss_and_grads). */
+/* A HIP stream at the device's highest (level < 0), default (0) or lowest (level > 0) dispatch priority.  Use 0: streams of different priorities
+ * have hung on this hardware.  The SPN step runs its 0.8 ms HBM-bound parameter update on such a stream beside the trunk's backward (host
+ * side: nets/spn.py loss_and_grads); a lower priority made no measurable difference. */
 int spb_stream_create(int level, spb_stream_t* out);
 int spb_stream_destroy(spb_stream_t stream);
 /* Stream fork without an event: everything enqueued on `to` after this call runs behind everything enqueued on `from` before it.
@@ -747,7 +747,8 @@ int spb_pack8_weight(int dtype, const void* W, long long ldw, int N, int K, unsi
 int spb_unpack8(int dtype, const unsigned char* codes, const unsigned char* scales, int block_rows, long long M, int K, void* Y, long long ldy,
                 spb_stream_t stream);
 /* y = act(x), and x packed (1 x 128) as the checkpoint of the backward pass;  dx = g * act'(value of the checkpoint).
- * act: SPB_ACT_GELU (x * Phi(x)), SPB_ACT_GELU_TANH (its tanh form), SPB_ACT_SILU (x / (1 + exp(-x))).  Y may be X, dX may be G. */
+ * act: SPB_ACT_GELU (x * Phi(x)), SPB_ACT_GELU_TANH (its tanh form), SPB_ACT_SILU (x / (1 + exp(-x))).  Y may be X, dX may be G.  Before the rounding to
+ * their type y is within 2^-21 |x|, dx within 2^-19 |g| of the functions (an absolute bound: far out on the negative side y has few digits). */
 enum { SPB_ACT_GELU = 4, SPB_ACT_GELU_TANH = 5, SPB_ACT_SILU = 6 };   /* spb_act8_* only */
 int spb_act8_fwd(int dtype, int act, const void* X, long long ldx, void* Y, long long ldy, long long M, int K, unsigned char* codes,
                  unsigned char* scales, spb_stream_t stream);

@@ -680,9 +680,8 @@ extern "C" int spb_debug_set_optim(int vec, int blocks, int nontemporal) {
 }
 #endif
 
-// Streams for work that must not compete with the launch stream for the compute units: level -1 = the device's highest
-// dispatch priority, 0 = default, +1 = lowest (the workgroup dispatcher serves higher-priority queues first, so a low stream's
-// long memory-bound kernel fills the slots the launch stream's kernels leave free instead of taking half the chip from them).
+// Streams beside the launch stream: level -1 = the device's highest dispatch priority, 0 = default, +1 = lowest.  The framework uses the default: streams of
+// different priorities have hung on this hardware, and the parameter update that once ran on a lower one gains nothing measurable from it.
 extern "C" int spb_stream_create(int level, spb_stream_t* out) {
   if (!out) return SPB_E_ARG;
   int least = 0, greatest = 0;

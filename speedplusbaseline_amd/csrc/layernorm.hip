@@ -332,7 +332,7 @@ __global__ __launch_bounds__(LN_JOIN * 64) void ln_join_kernel(const float* part
 }
 
 struct LnShape { int tpr, nv; };
-// the narrowest group that holds a row in 32 elements a thread
+// the narrowest group that holds a row in 16 (16 threads), 24 (64) or 32 (256) elements a thread
 inline LnShape ln_shape(int C) {
   if (C <= 128) return {16, 1};
   if (C <= 256) return {16, 2};
