@@ -6,12 +6,12 @@
 //
 // Both are bound by HBM: the forward reads x and writes y, the backward reads g and x and writes dx, each element once, because a row
 // stays in registers between its sums and its output.  The variance is taken from the differences to the mean, not from the sum of
-// squares: a row whose mean is far larger than its spread would lose the variance in the subtraction.  All sums are f32.
+// squares: a row whose mean is far larger than its spread would lose the variance in the subtraction.  Sums over a row are f32.
 //   * TPR threads share a row (16, 64 or 256), so that short rows fill a wave (four rows of up to 256 columns) and long rows need no second
 //     pass (8192 columns: 32 elements a thread).  Rows longer than that go through memory once per sum (ln_*_long).
 //   * Workgroups walk the rows with a stride, gamma and beta stay in registers, and the next row is requested before this one is summed.
-//   * dgamma / dbeta: a thread keeps its columns' sums in registers over its rows, the groups of a workgroup join through LDS, a workgroup
-//     stores one partial row, and a second launch adds the partial rows in order: no atomics, the same bits in every run.
+//   * dgamma / dbeta: a thread keeps its columns' sums in registers over its rows (f32), the groups of a workgroup join through LDS, a workgroup
+//     stores one partial row, and a second launch adds the partial rows in order, both in 64 bits: no atomics, the same bits in every run.
 #include "vec8.h"
 
 namespace {
@@ -242,10 +242,10 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const spb_layernorm_args_t 
           for (int i = 0; i < 8; ++i) join[grp * (TPR * NV * 8) + end.col(j, i)] = half ? db[j][i] : dg[j][i];
         __syncthreads();
         for (int c = threadIdx.x; c < C; c += 256) {
-          float v = 0.f;
+          double v = 0.;
 #pragma unroll
           for (int k = 0; k < GR; ++k) v += join[k * (TPR * NV * 8) + c];
-          out[half * C + c] = v;
+          out[half * C + c] = (float)v;
         }
       } else {
 #pragma unroll
@@ -283,13 +283,13 @@ __global__ __launch_bounds__(256) void ln_bwd_long(const spb_layernorm_args_t a)
   }
 }
 // partial rows of dgamma / dbeta for long rows: a thread a column, blockIdx.y a range of rows.  It runs BEFORE ln_bwd_long, whose output may
-// overwrite g.  Rows are added in blocks of 64, whose sums are added up: a single chain would collect a rounding for each of the range's rows.
+// overwrite g.  Rows are added in blocks of 64, whose sums are added up in 64 bits: a single chain would collect a rounding for each of the range's rows.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_cols(const spb_layernorm_args_t a, long long rows) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   const long long m0 = (long long)blockIdx.y * rows, m1 = m0 + rows < a.M ? m0 + rows : a.M;
   if (c >= a.C) return;
-  float dg = 0.f, db = 0.f;
+  double dg = 0., db = 0.;
   for (long long b = m0; b < m1; b += 64) {
     float pg = 0.f, pb = 0.f;
     for (long long m = b, e = b + 64 < m1 ? b + 64 : m1; m < e; ++m) {
@@ -300,34 +300,35 @@ __global__ __launch_bounds__(256) void ln_bwd_cols(const spb_layernorm_args_t a,
     dg += pg; db += pb;
   }
   float* out = a.part + (size_t)blockIdx.y * 2 * a.C;
-  out[c] = dg; out[a.C + c] = db;
+  out[c] = (float)dg; out[a.C + c] = (float)db;
 }
 
-// dgamma / dbeta (+)= the P partial rows, in order: 64 columns a workgroup, its sixteen waves a sixteenth of the rows each, eight requested at a time (a loop
-// of dependent additions waits for memory at every row: 128 rows took 35 us, this form takes 4)
+// dgamma / dbeta (+)= the P partial rows, in order and in 64 bits (0.6 us of 12 on 2351 x 1001, whose dgamma errs by 6.1e-8 of its norm instead of 1.3e-7): 64 columns a workgroup, its sixteen waves a
+// sixteenth of the rows each, eight requested at a time (a loop of dependent additions waits for memory at every row: 128 rows took 35 us, this form takes 4)
 constexpr int LN_JOIN = 16;
 __global__ __launch_bounds__(LN_JOIN * 64) void ln_join_kernel(const float* part, int P, int C, float* dgamma, float* dbeta, int accumulate) {
-  __shared__ float red[LN_JOIN][64];
+  __shared__ double red[LN_JOIN][64];
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const long long n = 2ll * C, c = (long long)blockIdx.x * 64 + l, cc = c < n ? c : n - 1;
   const int per = (P + LN_JOIN - 1) / LN_JOIN, p0 = w * per, p1 = p0 + per < P ? p0 + per : P;
-  float v = 0.f;
+  double v = 0.;
   for (int p = p0; p < p1; p += 8) {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = part[(p + i < p1 ? p + i : p1 - 1) * n + cc];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += p + i < p1 ? x[i] : 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = p + i < p1 ? x[i] : 0.f;
+    v += (((double)x[0] + x[1]) + ((double)x[2] + x[3])) + (((double)x[4] + x[5]) + ((double)x[6] + x[7]));
   }
   red[w][l] = v;
   __syncthreads();
   if (w == 0 && c < n) {
-    v = 0.f;
+    v = 0.;
 #pragma unroll
-    for (int k = 0; k < LN_JOIN; ++k) v += red[k][l];
+    for (int k = 0; k < LN_JOIN; k += 4) v += (red[k][l] + red[k + 1][l]) + (red[k + 2][l] + red[k + 3][l]);
     float* dst = c < C ? dgamma : dbeta;
     const int o = (int)(c < C ? c : c - C);
-    if (dst) dst[o] = (accumulate ? dst[o] : 0.f) + v;
+    if (dst) dst[o] = (accumulate ? dst[o] : 0.f) + (float)v;
   }
 }
 

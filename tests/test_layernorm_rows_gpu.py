@@ -27,3 +27,17 @@ def test_sums_over_many_long_rows(device, M, C, dtype):
     off_x = U * (x.double().abs() + mean.double().abs()) * rstd.double()[:, None]              # of x - mean
     assert ((dbeta.double() - want_b).abs() <= depth * U * want_b.abs()).all()
     assert ((dgamma.double() - want_g).abs() <= (depth + 3) * U * want_g.abs() + (M * g.double() * off_x)[0]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("M,C", [(8000, 64), (2000, 1001), (500, 4096), (1, 24)])
+def test_partial_sums_are_joined_without_further_roundings(device, M, C, dtype):
+    """At most 512 workgroups' worth of rows, all of them the same one: a thread has one term, so of dbeta only the partial rows and the result are rounded,
+    a rounding each (U * sum of the partial rows + U * result)."""
+    from speedplusbaseline_amd import ops
+    gen = torch.Generator().manual_seed(C)
+    x, g = torch.randn(1, C, generator=gen).to(dtype).cuda(), (1 + torch.rand(1, C, generator=gen)).to(dtype).cuda()
+    _, mean, rstd = ops.layernorm_fwd(x)
+    _, _, dbeta = ops.layernorm_bwd(g.expand(M, C), x.expand(M, C), mean.expand(M).contiguous(), rstd.expand(M).contiguous())
+    want = (M * g.double())[0]
+    assert ((dbeta.double() - want).abs() <= 2 * U * want * (1 + U)).all(), ((dbeta.double() - want).abs() / want).max() / U
