@@ -8,7 +8,8 @@
 //   * Tiles of dW: 256 x 256 with eight waves of 128 x 64, a stage requested ahead; 128 x 128, three stages ahead, with eight waves of 64 x 32; or
 //     64 x 64 with four waves of 32 x 32: a stage of the small tiles is multiplied in a fifth of the time that memory takes to answer.
 //     Stages of R rows (64; 32 with more than one piece in the larger tiles) in LDS, read with the transpose load ds_read_b64_tr_b16.
-//     The large tile is bound by LDS as much as by the products: 64 rows are 2048 clocks of matrix instructions, and 1536 of reads and 512 of writes in LDS.
+//     64 rows of the large tile are 2048 clocks of matrix instructions, and 1536 of reads and 512 of writes in LDS; the two hardly overlap (16384 x 4096 x 4096,
+//     counted: matrix cores busy 55 % of the time, LDS 35 %, bank conflicts 7 %).
 //   * bfloat16 gradients with 16-byte aligned rows go to LDS by DMA, the others through registers.
 //   * Of the two waves on a SIMD one multiplies a stage before it brings the next one into place, the other after it: the matrix cores work while operands are
 //     converted (16384 x 4096 x 4096: 459 -> 427 us; 37632 x 1024 x 1280: 183 -> 174).
