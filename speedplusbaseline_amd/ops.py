@@ -548,8 +548,8 @@ def dequant8(P, dtype=torch.bfloat16, Y=None):
 
 
 def gemm8(A, B, bias=None, dtype=torch.bfloat16, Y=None):
-    """Y [M, N] = A [M, K] (quant8) times the transpose of B [N, K] (quant8_weight or quant8) + bias (float32 [N]).  dtype float32: the products run
-    through the bfloat16 matrix instructions, where they are exact; 16-bit types: through the 8-bit ones."""
+    """Y [M, N] = A [M, K] (quant8) times the transpose of B [N, K] (quant8_weight or quant8) + bias (float32 [N]).  dtype float32, or up to
+    16 rows: the products run through the bfloat16 matrix instructions, where they are exact; otherwise through the 8-bit ones."""
     dev, aq, a_s = _packed(A, "A", None, 1)
     _, bq, bs = _packed(B, "B", dev)
     if A.K != B.K:

@@ -68,3 +68,15 @@ def test_wgrad_of_infinite_gradients(device, M, N, K, dtype):
     assert want[2].isinf().any() and want[5].isnan().any() and want[7].isnan().all()
     for f in (torch.isnan, torch.isposinf, torch.isneginf):
         assert torch.equal(f(dw), f(want)), f.__name__
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (16, 513, 1001), (5, 40, 17000), (2, 16, 64)])
+def test_few_rows_have_exact_products(device, M, N, K, dtype):
+    """a 16-bit result of up to 16 rows is the float32 one rounded once"""
+    from speedplusbaseline_amd import ops
+    A, (B, _) = ops.quant8(data(M, K, torch.bfloat16, M, scale=0.02)), ops.quant8_weight(data(N, K, torch.float32, N, scale=0.02), transpose=False)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(2)).cuda()
+    y = ops.gemm8(A, B, bias=bias, dtype=torch.float32)
+    check_product(A, B, bias, y)
+    assert torch.equal(ops.gemm8(A, B, bias=bias, dtype=dtype), y.to(dtype))
