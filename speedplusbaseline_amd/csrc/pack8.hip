@@ -237,28 +237,30 @@ inline bool bad_dtype(int d) { return d != SPB_F32 && d != SPB_BF16; }
   } while (0)
 
 // as many rows a launch as it has threads for (16 a block; 8 elements each)
-template <int ACT> int pack_rows(int dtype, RowArgs a, long long M, hipStream_t s) {
-  if (M * a.KB > 0xfffffff0ll) return SPB_E_SHAPE;
-  const long long most = (P8_THREADS / 256 * 16) / a.KB, es = dtype == SPB_F32 ? 4 : 2;
-  for (; M > 0; M -= most) {
-    a.blocks = (unsigned)((M < most ? M : most) * a.KB);
+template <int ACT> int pack_rows(int dtype, const RowArgs& all, long long M, hipStream_t s) {
+  if (M * all.KB > 0xfffffff0ll) return SPB_E_SHAPE;
+  const long long most = (P8_THREADS / 256 * 16) / all.KB, es = dtype == SPB_F32 ? 4 : 2;
+  for (long long m = 0; m < M; m += most) {
+    RowArgs a = all;
+    a.blocks = (unsigned)((M - m < most ? M - m : most) * a.KB);
+    a.X = (const char*)a.X + m * a.ldx * es; a.Q += m * a.Kp; a.S += m * a.Sp;
+    if (ACT != 0) a.Y = (char*)a.Y + m * a.ldy * es;
     P8_LAUNCH(pack8_rows_kernel, dim3(a.blocks / 16 + (a.blocks % 16 ? 1 : 0)), ACT);
-    a.X = (const char*)a.X + most * a.ldx * es; a.Q += most * a.Kp; a.S += most * a.Sp;
-    if (ACT != 0) a.Y = (char*)a.Y + most * a.ldy * es;
   }
   return 0;
 }
-template <int ACT> int unpack(int dtype, UnpackArgs a, long long M, hipStream_t s) {
-  if (M * a.V > 0xfffffff0ll) return SPB_E_SHAPE;
-  long long most = (P8_THREADS / 256 * 256) / a.V;
+template <int ACT> int unpack(int dtype, const UnpackArgs& all, long long M, hipStream_t s) {
+  if (M * all.V > 0xfffffff0ll) return SPB_E_SHAPE;
+  long long most = (P8_THREADS / 256 * 256) / all.V;
   const long long es = dtype == SPB_F32 ? 4 : 2;
-  if (most < M && a.shift) most = most >> 7 << 7;       // whole blocks of rows
+  if (most < M && all.shift) most = most >> 7 << 7;       // whole blocks of rows
   if (most == 0) return SPB_E_SHAPE;
-  for (; M > 0; M -= most) {
-    a.vecs = (unsigned)((M < most ? M : most) * a.V);
+  for (long long m = 0; m < M; m += most) {
+    UnpackArgs a = all;
+    a.vecs = (unsigned)((M - m < most ? M - m : most) * a.V);
+    a.Q += m * a.Kp; a.S += (m >> a.shift) * a.Sp; a.Y = (char*)a.Y + m * a.ldy * es;
+    if (ACT != 0) a.G = (const char*)a.G + m * a.ldg * es;
     P8_LAUNCH(unpack8_kernel, dim3(a.vecs / 256 + (a.vecs % 256 ? 1 : 0)), ACT);
-    a.Q += most * a.Kp; a.S += (most >> a.shift) * a.Sp; a.Y = (char*)a.Y + most * a.ldy * es;
-    if (ACT != 0) a.G = (const char*)a.G + most * a.ldg * es;
   }
   return 0;
 }
