@@ -716,7 +716,7 @@ typedef struct spb_layernorm_args {
   float* rstd;         /* [M] */
   float* dgamma;       /* backward: [C] or NULL: sum over rows of g * (x - mean) * rstd */
   float* dbeta;        /* backward: [C] or NULL: sum over rows of g; not dgamma's buffer.  Both sums are f32 over a thread's
-                        * rows (at most M / 512 additions), 64 bits beyond that, and rounded to f32 */
+                        * rows (at most 64 or M / 512 additions), 64 bits beyond that, and rounded to f32 */
   float* part;         /* backward with dgamma or dbeta: workspace of spb_layernorm_bwd_floats(M, C) floats */
   long long part_cap;  /* floats available at `part` */
   long long M, ldx, ldg, ldy;

@@ -365,7 +365,7 @@ inline bool by_rows(long long M, int N) { return M <= 16 && p8_fits((N + 15) / 1
 // 2048 x 4096 x 2048 27 / 19, f32 16384 x 2304 x 4096 306 / 274, f32 300 x 40000 x 1024 78 / 41.
 // f32 with a side of at most 64 takes 64 x 64 tiles, which convert nothing that is not used (150528 x 24 x 144: 20.5 us, 128: 22.9; 37632 x 64 x 1024 16.3 / 21.4; 16-bit
 // results gain nothing: 13.9 / 13.8, 11.2 / 10.7).
-// Smaller products take 64 x 64 tiles (2048 x 1024 x 1024, 128 tiles of 128: 7.0 us against 8.3), and where even these are fewer than 256 the reduction is split into parts of at least four
+// Smaller products take 64 x 64 tiles (2048 x 1024 x 1024, 128 tiles of 128: 7.0 us against 8.3; 2352 x 1024 x 1024, 152 tiles: 10.1 against 8.4), and where even these are fewer than 256 the reduction is split into parts of at least four
 // steps, whose sums a second launch adds up, if the steps saved (0.29 us each) are
 // worth that launch (3.5 us) and the partial sums' way out and back at 3.5 TB/s: 48 x 4096 x 9216 in four parts 12.4 us, in one 21.7, 300 x 512 x 4096 9.3 and
 // 11.1, but 4096 x 128 x 1024 in two parts 9.2, in one 5.1.
