@@ -101,7 +101,7 @@ def build(force=False, verbose=True):
 
     srcs16 = [os.path.join(CSRC, s) for s in SOURCES_F16]
     srcsdet = [os.path.join(CSRC, s) for s in SOURCES_DET]
-    with ThreadPoolExecutor(max_workers=4) as ex:
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 4)) as ex:
         objs = list(ex.map(compile_one, srcs))
         objs16 = list(ex.map(lambda s_: compile_twin(s_, "f16", "-DSPB_F16"), srcs16))
         objsdet = list(ex.map(lambda s_: compile_twin(s_, "det", "-DSPB_DET"), srcsdet))
